@@ -22,7 +22,10 @@ v_cached, wq, wk, wv, wo, bq, bk, bv, bo, use_bias, n_head, n_head_kv,
 n_embd, rope_freq_base, rope_freq_scale)``, the paged KV cache
 (``kvcache_gather``, ``kvcache_scatter_decode``, ``kvcache_scatter_prefill``)
 and ``AttentionBlockDecode`` (packed weights; ``.paged`` reads the paged
-cache in place),
+cache in place), and the cache in 8 bits: ``QuantizedKVPool`` (e4m3 codes, one
+scale per block and head), ``kvcache_append`` (new tokens rotated and written
+into their pages) and ``attention_paged`` (decode steps, chunks and prompts
+over it),
 
 plus ``router``, ``permute``, ``pack_expert_weights``,
 ``quantize_expert_weights``, ``QuantizedExpertWeights``,
@@ -62,6 +65,11 @@ from .attention import (  # noqa: F401
     kvcache_scatter_decode,
     kvcache_scatter_prefill,
     pack_linear_weights,
+)
+from .paged import (  # noqa: F401
+    QuantizedKVPool,
+    attention_paged,
+    kvcache_append,
 )
 from . import _lib as lowlevel  # noqa: F401
 from . import params  # noqa: F401
@@ -113,6 +121,9 @@ __all__ = [
     "kvcache_gather",
     "kvcache_scatter_decode",
     "kvcache_scatter_prefill",
+    "QuantizedKVPool",
+    "kvcache_append",
+    "attention_paged",
     "ATTN_HPARAMS",
     "AttentionHParams",
     "AttentionLayer",

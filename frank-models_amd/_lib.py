@@ -157,6 +157,19 @@ SIGNATURES = {
          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_float, _c_int, _vp, _vp, _vp, _vp, _sz,
          _vp],
     ),
+    # caches of e4m3 codes
+    "fmoe_kvcache_append": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _c_i64,
+         _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, ctypes.c_float,
+         ctypes.c_float, _vp],
+    ),
+    "fmoe_attention_paged_workspace_bytes": (_sz, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
+    "fmoe_attention_paged": (
+        _c_int,
+        [_vp, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_int, ctypes.c_float, _c_int, _vp, _vp, _sz, _vp],
+    ),
 }
 
 _lock = threading.Lock()

@@ -1579,6 +1579,165 @@ int fmoe_attention_sublayer_decode_paged(const void* residual, const void* attn_
                          rope_freq_scale, act_dtype, out, k_new, v_new, workspace, workspace_bytes, stream);
 }
 
+// ------------------------------------------------------------ caches of e4m3 codes
+// Shapes and pointers shared by the append and the attention over pages.
+static int check_pages(int64_t n_blocks, int64_t block_size, int64_t n_head_kv, int64_t head_dim, int64_t layer,
+                       int64_t n_layers, int64_t batch, int64_t seq_len, int64_t max_blocks_per_seq) {
+  FMOE_TRY(check_pool(n_blocks, block_size));
+  FMOE_TRY(check_dims("n_head_kv", n_head_kv, 1, 65535));
+  if (!paged_attn_supported(static_cast<int>(std::min<int64_t>(head_dim, kMaxDim))))
+    return fail(FMOE_ERR_SHAPE, "head_dim %lld is not supported (16/32/64/128)", static_cast<long long>(head_dim));
+  FMOE_TRY(check_dims("n_layers", n_layers, 1, kMaxDim));
+  FMOE_TRY(check_dims("layer", layer, 0, n_layers - 1));
+  FMOE_TRY(check_dims("batch", batch, 0, 65535));
+  FMOE_TRY(check_dims("seq_len", seq_len, 0, kMaxDim));
+  FMOE_TRY(check_dims("max_blocks_per_seq", max_blocks_per_seq, 1, kMaxDim));
+  return FMOE_OK;
+}
+
+// A [batch, seq_len, heads, head_dim] operand: token stride and 16-byte rows.
+static int check_tokens(const char* what, const void* p, int64_t stride, int64_t heads, int64_t head_dim, int dtype) {
+  if (!p) return fail(FMOE_ERR_INVALID_ARGUMENT, "null %s", what);
+  if (stride < heads * head_dim)
+    return fail(FMOE_ERR_SHAPE, "%s: token stride %lld < %lld elements", what, static_cast<long long>(stride),
+                static_cast<long long>(heads * head_dim));
+  if (reinterpret_cast<uintptr_t>(p) % 16 || stride * dtype_bytes(dtype) % 16)
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: tokens must be 16-byte aligned", what);
+  return FMOE_OK;
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int fmoe_kvcache_append(void* k_cache, void* v_cache, float* k_scales, float* v_scales, int cache_dtype,
+                        int64_t n_blocks, int64_t block_size, int64_t n_head_kv, int64_t head_dim, int64_t layer,
+                        const void* k, int64_t k_stride, const void* v, int64_t v_stride, const void* q,
+                        int64_t q_stride, void* q_out, int64_t q_out_stride, int64_t n_head, int act_dtype,
+                        int64_t batch, int64_t seq_len, const int32_t* block_tables, int64_t n_layers,
+                        int64_t max_blocks_per_seq, const int32_t* start_positions, const int32_t* seq_lens, int rope,
+                        float rope_freq_base, float rope_freq_scale, void* stream) {
+  if (!act_dtype_ok(act_dtype)) return fail(FMOE_ERR_DTYPE, "activation dtype %d", act_dtype);
+  if (cache_dtype != act_dtype && cache_dtype != FMOE_F8E4M3FN)
+    return fail(FMOE_ERR_DTYPE, "cache dtype %d with activation dtype %d", cache_dtype, act_dtype);
+  FMOE_TRY(check_pages(n_blocks, block_size, n_head_kv, head_dim, layer, n_layers, batch, seq_len,
+                       max_blocks_per_seq));
+  if (q) FMOE_TRY(check_dims("n_head", n_head, 1, 65535));
+  if (rope != 0 && rope != 1) return fail(FMOE_ERR_INVALID_ARGUMENT, "rope must be 0 or 1");
+  if (rope && !(rope_freq_base > 0.f && std::isfinite(rope_freq_base) && std::isfinite(rope_freq_scale)))
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "rope_freq_base must be positive and finite, rope_freq_scale finite");
+  if (batch == 0 || seq_len == 0) return ok();
+  if (!k_cache || !v_cache || !block_tables || !start_positions)
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "null pointer");
+  const bool codes = cache_dtype == FMOE_F8E4M3FN;
+  if (codes && (!k_scales || !v_scales)) return fail(FMOE_ERR_INVALID_ARGUMENT, "a cache of codes needs scales");
+  if (!aligned16(k_cache) || !aligned16(v_cache))
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "K/V pools must be 16-byte aligned");
+  FMOE_TRY(check_tokens("k", k, k_stride, n_head_kv, head_dim, act_dtype));
+  FMOE_TRY(check_tokens("v", v, v_stride, n_head_kv, head_dim, act_dtype));
+  if (q) {
+    FMOE_TRY(check_tokens("q", q, q_stride, n_head, head_dim, act_dtype));
+    FMOE_TRY(check_tokens("q_out", q_out, q_out_stride, n_head, head_dim, act_dtype));
+  }
+  FMOE_TRY(ensure_device());
+  KvAppendArgs a{};
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.k = k;
+  a.v = v;
+  a.q = q;
+  a.q_out = q_out;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_stride = q_stride;
+  a.q_out_stride = q_out_stride;
+  a.tables = block_tables + layer * batch * max_blocks_per_seq;
+  a.start = start_positions;
+  a.lens = seq_lens;
+  a.n_blocks = n_blocks;
+  a.block_size = static_cast<int>(block_size);
+  a.max_blocks = static_cast<int>(max_blocks_per_seq);
+  a.batch = static_cast<int>(batch);
+  a.seq_len = static_cast<int>(seq_len);
+  a.n_head = static_cast<int>(n_head);
+  a.n_head_kv = static_cast<int>(n_head_kv);
+  while ((1 << a.log2_dim) < head_dim) ++a.log2_dim;
+  a.rope = rope;
+  a.log2_base = rope ? std::log2(static_cast<double>(rope_freq_base)) : 0.;
+  a.freq_scale = rope_freq_scale;
+  FMOE_HIP(launch_kv_append(a, act_dtype, codes, static_cast<hipStream_t>(stream)));
+  return ok();
+}
+
+size_t fmoe_attention_paged_workspace_bytes(int64_t batch, int64_t seq_len, int64_t max_context_len, int64_t n_head,
+                                            int64_t n_head_kv, int64_t head_dim, int act_dtype) {
+  if (!act_dtype_ok(act_dtype) || batch < 0 || batch > 65535 || seq_len < 0 || seq_len > kMaxDim ||
+      max_context_len < 0 || max_context_len > kMaxDim || n_head_kv < 1 || n_head_kv > n_head || n_head > 65535 ||
+      n_head % n_head_kv || !paged_attn_supported(static_cast<int>(std::min<int64_t>(head_dim, kMaxDim))))
+    return 0;
+  return align_up(paged_attn_workspace_floats(static_cast<int>(batch), static_cast<int>(seq_len),
+                                              static_cast<int>(max_context_len), static_cast<int>(n_head),
+                                              static_cast<int>(n_head_kv), static_cast<int>(head_dim), act_dtype) *
+                  sizeof(float));
+}
+
+int fmoe_attention_paged(const void* q, int64_t q_stride, const void* k_cache, const float* k_scales,
+                         const void* v_cache, const float* v_scales, int64_t n_blocks, int64_t block_size,
+                         int64_t layer, const int32_t* block_tables, const int32_t* context_lens,
+                         const int32_t* seq_lens, int64_t n_layers, int64_t batch, int64_t seq_len,
+                         int64_t max_blocks_per_seq, int64_t max_context_len, int64_t n_head, int64_t n_head_kv,
+                         int64_t head_dim, int causal, float scale, int act_dtype, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  if (!act_dtype_ok(act_dtype)) return fail(FMOE_ERR_DTYPE, "activation dtype %d", act_dtype);
+  FMOE_TRY(check_pages(n_blocks, block_size, n_head_kv, head_dim, layer, n_layers, batch, seq_len,
+                       max_blocks_per_seq));
+  FMOE_TRY(check_dims("n_head", n_head, n_head_kv, 65535));
+  if (n_head % n_head_kv) return fail(FMOE_ERR_SHAPE, "n_head %% n_head_kv != 0");
+  FMOE_TRY(check_dims("max_context_len", max_context_len, 0, kMaxDim));
+  if (seq_len > 0) FMOE_TRY(check_dims("seq_len * n_head", seq_len, 0, kMaxDim / n_head));
+  if (causal != 0 && causal != 1) return fail(FMOE_ERR_INVALID_ARGUMENT, "causal must be 0 or 1");
+  if (!(scale >= 0.f && std::isfinite(scale)))
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "scale must be positive and finite (0: 1/sqrt(head_dim))");
+  if (batch == 0 || seq_len == 0) return ok();
+  if (!k_cache || !v_cache || !k_scales || !v_scales || !block_tables || !context_lens || !out)
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned16(k_cache) || !aligned16(v_cache))
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "K/V pools must be 16-byte aligned");
+  if (!aligned16(out)) return fail(FMOE_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned");
+  FMOE_TRY(check_tokens("q", q, q_stride, n_head, head_dim, act_dtype));
+  const size_t need = fmoe_attention_paged_workspace_bytes(batch, seq_len, max_context_len, n_head, n_head_kv,
+                                                           head_dim, act_dtype);
+  if (need) FMOE_TRY(check_workspace(workspace, workspace_bytes, need));
+  FMOE_TRY(ensure_device());
+  PagedAttnArgs a{};
+  a.q = q;
+  a.q_stride = q_stride;
+  a.q_dtype = act_dtype;
+  a.out_dtype = act_dtype;
+  a.k_pool = static_cast<const uint8_t*>(k_cache);
+  a.v_pool = static_cast<const uint8_t*>(v_cache);
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.tables = block_tables + layer * batch * max_blocks_per_seq;
+  a.ctx_lens = context_lens + layer * batch;
+  a.lens = seq_lens;
+  a.n_blocks = n_blocks;
+  a.block_size = static_cast<int>(block_size);
+  a.max_blocks = static_cast<int>(max_blocks_per_seq);
+  a.max_ctx = static_cast<int>(max_context_len);
+  a.batch = static_cast<int>(batch);
+  a.seq_len = static_cast<int>(seq_len);
+  a.n_head = static_cast<int>(n_head);
+  a.n_head_kv = static_cast<int>(n_head_kv);
+  a.head_dim = static_cast<int>(head_dim);
+  a.causal = causal;
+  a.scale = scale > 0.f ? scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(head_dim)));
+  a.out = out;
+  a.part = static_cast<float*>(workspace);
+  FMOE_HIP(launch_paged_attn(a, static_cast<hipStream_t>(stream)));
+  return ok();
+}
+
 }  // extern "C"
 
 // Shared by the paged attention and the attention sub-layer: norm_w non-null

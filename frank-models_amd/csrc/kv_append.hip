@@ -1,0 +1,286 @@
+// Appending new tokens to a paged K/V cache, with the rotary position applied
+// on the way: keys are rotated and written with the values into the pages of
+// their sequence, queries are rotated with the same angles.
+//
+// Pool pages [n_blocks, block_size, n_head_kv, head_dim] hold either the
+// activations' type or e4m3 codes with one scale for each (page, head).  With
+// codes, the values x of an append to rows [r0, r1) of a page and a head set
+//   S' = max(S, s(max |x|)) for r0 > 0 (the page holds earlier rows at S),
+//   S' = s(max |x|)         for r0 = 0 (a page begun anew),
+// where s(a) is the least power of two with a <= 448 s(a); rows below r0 are
+// rounded again from S to S' where S' > S, the new rows are e4m3(x / S').
+// Powers of two make the second rounding exact but for what falls below the
+// codes' smallest normal value, 2^-15 of the page's largest.
+#include "common.h"
+#include "launch.h"
+
+namespace fmoe {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kVec = 8;           // elements of a lane's load
+constexpr int kBatch = 4;         // loads of a lane in flight
+constexpr int kAngleFloats = 8192;  // LDS for (cos, sin): rows of a chunk x head_dim
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = a[i];
+      x[4 + i] = b[i];
+    }
+  } else {
+    const u32x4_t a = *reinterpret_cast<const u32x4_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = bf16_lo(a[i]);
+      x[2 * i + 1] = bf16_hi(a[i]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4_t*>(p) = f32x4_t{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{x[4], x[5], x[6], x[7]};
+  } else {
+    *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+                                             pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+  }
+}
+
+// Eight values times inv as codes, round to nearest even; what is not finite
+// becomes NaN (v_cvt_pk_fp8_f32 gives NaN beyond 464, and finite values are
+// within 448 of the scale that inv inverts).
+__device__ __forceinline__ u32x2_t codes8(const float* x, float inv) {
+  uint32_t w[2];
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * d] * inv, x[4 * d + 1] * inv, 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * d + 2] * inv, x[4 * d + 3] * inv, c, true);
+    w[d] = static_cast<uint32_t>(c);
+  }
+  return u32x2_t{w[0], w[1]};
+}
+
+__device__ __forceinline__ void values8(u32x2_t c, float* x) {
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[d]), false);
+    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[d]), true);
+    x[4 * d] = lo[0];
+    x[4 * d + 1] = lo[1];
+    x[4 * d + 2] = hi[0];
+    x[4 * d + 3] = hi[1];
+  }
+}
+
+// The page of position 0 rounded down also for positions before the sequence.
+__device__ __forceinline__ int64_t first_page(int start, int block_size) {
+  return start >= 0 ? start / block_size : -((-static_cast<int64_t>(start) + block_size - 1) / block_size);
+}
+
+// The new tokens [lo, hi) of a sequence from `start` that lie in its page lp.
+__device__ __forceinline__ void page_tokens(int64_t lp, int start, int seq_len, int block_size, int& lo, int& hi) {
+  const int64_t first = lp * block_size - start;
+  lo = static_cast<int>(first > 0 ? min(first, static_cast<int64_t>(seq_len)) : 0);
+  hi = static_cast<int>(min(max(first + block_size, static_cast<int64_t>(0)), static_cast<int64_t>(seq_len)));
+}
+
+// Block (page of the new tokens, group of heads, sequence).  An item is one
+// K, V or Q head of the page's new tokens; a wave takes an item, so a head's
+// maximum needs no barrier.  Bound by memory; for a decode step's few tokens
+// by one round trip after another (start, table entry, page scale).
+// T: activations.  C: codes (the pool holds e4m3), else the pool holds T.
+template <typename T, bool C>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float2 angles[];  // [rows of a chunk][D / 2]
+  const int b = blockIdx.z, x = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int D = 1 << a.log2_dim, bs = a.block_size;
+  const int start = a.start[b];
+  const int len = a.lens ? min(max(a.lens[b], 0), a.seq_len) : a.seq_len;  // tokens that are cached
+  const int64_t lp = first_page(start, bs) + x;
+  int s0, s1;
+  page_tokens(lp, start, a.seq_len, bs, s0, s1);
+  if (s0 >= s1) return;
+  const int n = s1 - s0, n_kv = min(len, s1) - s0;
+  const int r0 = static_cast<int>(static_cast<int64_t>(start) + s0 - lp * bs);
+
+  // The page, and whether a later append of this call names it too: then that
+  // one alone writes it.
+  int64_t page = -1;
+  if (n_kv > 0 && lp >= 0 && lp < a.max_blocks) {
+    page = a.tables[static_cast<int64_t>(b) * a.max_blocks + lp];
+    if (page >= a.n_blocks) page = -1;
+  }
+  bool later = false;
+  if (page >= 0) {
+    const int64_t count = static_cast<int64_t>(a.batch - b) * a.pages;
+    for (int64_t i = x + 1 + tid; i < count; i += kThreads) {
+      const int b2 = b + static_cast<int>(i / a.pages);
+      const int st2 = a.start[b2];
+      const int64_t lp2 = first_page(st2, bs) + i % a.pages;
+      if (lp2 < 0 || lp2 >= a.max_blocks) continue;
+      int lo, hi;
+      page_tokens(lp2, st2, a.seq_len, bs, lo, hi);
+      if (lo >= hi || (a.lens && lo >= a.lens[b2])) continue;
+      later |= a.tables[static_cast<int64_t>(b2) * a.max_blocks + lp2] == page;
+    }
+  }
+  const bool write = !__syncthreads_or(later) && page >= 0;
+
+  const int items = 2 * a.n_head_kv + (a.q ? a.n_head : 0);
+  const int log2_vecs = a.log2_dim - 3;  // loads of a row
+  const int chunk = min(n, kAngleFloats >> a.log2_dim);
+  const int64_t row_elems = static_cast<int64_t>(a.n_head_kv) << a.log2_dim;
+  bool have_angles = false;
+
+  for (int i0 = blockIdx.y * kWaves; i0 < items; i0 += gridDim.y * kWaves) {
+    const int item = i0 + wave;
+    const bool active = item < items;
+    const int kind = item < a.n_head_kv ? 0 : item < 2 * a.n_head_kv ? 1 : 2;  // k, v, q
+    const int head = kind == 0 ? item : kind == 1 ? item - a.n_head_kv : item - 2 * a.n_head_kv;
+    const bool turn = a.rope && kind != 1;
+    const int rows = !active ? 0 : kind == 2 ? n : write ? n_kv : 0;
+    const int64_t stride = kind == 0 ? a.k_stride : kind == 1 ? a.v_stride : a.q_stride;
+    const T* src = static_cast<const T*>(kind == 0 ? a.k : kind == 1 ? a.v : a.q) +
+                   (static_cast<int64_t>(b) * a.seq_len + s0) * stride + (static_cast<int64_t>(head) << a.log2_dim);
+    float amax = 0.f, inv = 0.f;
+    float v[kBatch][kVec];
+
+    // Two passes over the rows of a K or V item with codes (maximum, then
+    // codes), one otherwise.
+    for (int pass = C ? 0 : 1; pass < 2; ++pass) {
+      for (int c0 = 0; c0 < n; c0 += chunk) {
+        const int c1 = min(c0 + chunk, n);
+        if (a.rope && (!have_angles || chunk < n)) {  // block-uniform
+          if (have_angles) __syncthreads();
+          // A thread keeps one pair and steps through rows: angles in 64 bits,
+          // the row's turned on by the step's with a complex product.
+          const int pairs = D / 2, i = tid & (pairs - 1), step = kThreads >> (a.log2_dim - 1);
+          const double freq = a.freq_scale * exp2(-static_cast<double>(2 * i) / D * a.log2_base);
+          const int r = tid >> (a.log2_dim - 1);
+          double sn, cs, dsn = 0., dcs = 1.;
+          sincos(static_cast<double>(static_cast<int64_t>(start) + s0 + c0 + r) * freq, &sn, &cs);
+          if (r + step < c1 - c0) sincos(static_cast<double>(step) * freq, &dsn, &dcs);
+          for (int row = r; row < c1 - c0; row += step) {
+            angles[row * pairs + i] = float2{static_cast<float>(cs), static_cast<float>(sn)};
+            const double t = cs * dcs - sn * dsn;
+            sn = sn * dcs + cs * dsn;
+            cs = t;
+          }
+          have_angles = true;
+          __syncthreads();
+        }
+        const int vecs = max(min(c1, rows) - c0, 0) << log2_vecs;
+        if (pass == 0 && kind == 2) continue;
+        const bool kept = C && kind != 2 && pass == 1 && rows <= chunk && vecs <= kBatch * kWave;  // v holds the rows
+        for (int e0 = 0; e0 < vecs; e0 += kBatch * kWave) {
+          if (!kept) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+              const int e = e0 + u * kWave + lane;
+              if (e < vecs)
+                load8(src + (c0 + (e >> log2_vecs)) * stride + ((e & ((1 << log2_vecs) - 1)) << 3), v[u]);
+            }
+            if (turn) {
+#pragma unroll
+              for (int u = 0; u < kBatch; ++u) {
+                const int e = e0 + u * kWave + lane;
+                if (e < vecs) {
+                  // row e >> log2_vecs, pairs from 4 * (e's load of the row): 4 e in all
+                  const float2* cs = angles + 4 * e;
+#pragma unroll
+                  for (int p = 0; p < 4; ++p) rope_apply(v[u][2 * p], v[u][2 * p + 1], cs[p], v[u][2 * p], v[u][2 * p + 1]);
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int e = e0 + u * kWave + lane;
+            if (e >= vecs) continue;
+            if (pass == 0) {
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) {
+                const float m = fabsf(v[u][k]);
+                amax = fmaxf(amax, m < INFINITY ? m : 0.f);
+              }
+              continue;
+            }
+            const int row = c0 + (e >> log2_vecs), col = (e & ((1 << log2_vecs) - 1)) << 3;
+            if (kind == 2) {
+              store8(static_cast<T*>(a.q_out) + (static_cast<int64_t>(b) * a.seq_len + s0 + row) * a.q_out_stride +
+                         (static_cast<int64_t>(head) << a.log2_dim) + col,
+                     v[u]);
+              continue;
+            }
+            const int64_t at = (page * bs + r0 + row) * row_elems + (static_cast<int64_t>(head) << a.log2_dim) + col;
+            void* pool = kind == 0 ? a.k_cache : a.v_cache;
+            if constexpr (C)
+              *reinterpret_cast<u32x2_t*>(static_cast<f8_t*>(pool) + at) = codes8(v[u], inv);
+            else
+              store8(static_cast<T*>(pool) + at, v[u]);
+          }
+        }
+      }
+      if constexpr (C) {
+        if (pass == 0 && kind != 2 && rows > 0) {  // wave-uniform
+          amax = wave_max(amax);
+          float scale = amax > 0.f ? pow2_scale(amax, &inv) : 0x1p-126f;
+          float* at = (kind == 0 ? a.k_scales : a.v_scales) + page * a.n_head_kv + head;
+          if (r0 > 0) {
+            const float old = *at;
+            if (scale > old) {
+              const float f = old / scale;
+              f8_t* pool = static_cast<f8_t*>(kind == 0 ? a.k_cache : a.v_cache) + page * bs * row_elems +
+                           (static_cast<int64_t>(head) << a.log2_dim);
+              for (int e = lane; e < r0 << log2_vecs; e += kWave) {
+                u32x2_t* p = reinterpret_cast<u32x2_t*>(pool + (e >> log2_vecs) * row_elems +
+                                                        ((e & ((1 << log2_vecs) - 1)) << 3));
+                float y[kVec];
+                values8(*p, y);
+                *p = codes8(y, f);
+              }
+            } else {
+              scale = old;
+            }
+          }
+          inv = 1.f / scale;
+          if (lane == 0) *at = scale;
+        }
+      }
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_kv_append(const KvAppendArgs& args, int act, bool codes, hipStream_t s) {
+  KvAppendArgs a = args;
+  if (a.batch == 0 || a.seq_len == 0) return hipSuccess;
+  // pages that seq_len tokens from any start can touch
+  const int64_t pages = (static_cast<int64_t>(a.seq_len) + a.block_size - 2) / a.block_size + 1;
+  a.pages = static_cast<int>(pages);
+  const int items = 2 * a.n_head_kv + (a.q ? a.n_head : 0);
+  const int groups = (items + kWaves - 1) / kWaves;
+  const int rows = min(min(a.block_size, a.seq_len), kAngleFloats >> a.log2_dim);
+  const size_t lds = a.rope ? (static_cast<size_t>(rows) << a.log2_dim) * sizeof(float) : 0;
+  const dim3 grid(static_cast<unsigned>(pages), groups, a.batch);
+  if (act == DT_F32 && codes)
+    hipLaunchKernelGGL((kv_append_kernel<float, true>), grid, dim3(kThreads), lds, s, a);
+  else if (act == DT_F32)
+    hipLaunchKernelGGL((kv_append_kernel<float, false>), grid, dim3(kThreads), lds, s, a);
+  else if (codes)
+    hipLaunchKernelGGL((kv_append_kernel<bf16_t, true>), grid, dim3(kThreads), lds, s, a);
+  else
+    hipLaunchKernelGGL((kv_append_kernel<bf16_t, false>), grid, dim3(kThreads), lds, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace fmoe

@@ -406,4 +406,59 @@ hipError_t launch_attn_decode(const float* q_rot, const void* k_pool, const void
                               int head_dim, int dtype, float scale, float* part, void* out, hipStream_t s,
                               const KvScatterDecode* scatter = nullptr);
 
+// ---- append to a paged cache (kv_append.hip)
+// Token (b, s) of k, v [n_head_kv, head_dim] and q [n_head, head_dim] starts
+// at (b * seq_len + s) * stride elements; k and q are rotated (rope) at
+// position start[b] + s, k and v of tokens s < lens[b] (null: all) go to
+// their pages, q to q_out (q may be null).  16-byte aligned rows.
+struct KvAppendArgs {
+  void* k_cache;  // [n_blocks, block_size, n_head_kv, head_dim]
+  void* v_cache;
+  float* k_scales;  // [n_blocks, n_head_kv], pools of codes only
+  float* v_scales;
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  int64_t k_stride, v_stride, q_stride, q_out_stride;
+  const int* tables;  // [batch, max_blocks] (this layer)
+  const int* start;   // [batch]
+  const int* lens;    // [batch] or null
+  int64_t n_blocks;
+  int block_size, max_blocks, batch, seq_len, n_head, n_head_kv, log2_dim;
+  int pages;  // set by the launcher: pages that a sequence's new tokens can touch
+  int rope;
+  double log2_base, freq_scale;
+};
+hipError_t launch_kv_append(const KvAppendArgs& args, int act, bool codes, hipStream_t s);
+
+// ---- attention over e4m3 pages (attention_paged.hip)
+// Query (b, s, h) at ((b * seq_len + s) * q_stride + h * head_dim), one of the
+// last lens[b] (null: seq_len) tokens of a context of ctx_lens[b] + ctx_add,
+// against positions below min(context, max_ctx) and, causal, up to its own.
+// zero_to: positions from the context's end to it are keys and values of
+// zeros that every query attends (0: none).
+struct PagedAttnArgs {
+  const void* q;
+  int64_t q_stride;
+  int q_dtype, out_dtype;
+  const uint8_t* k_pool;  // [n_blocks, block_size, n_head_kv, head_dim]
+  const uint8_t* v_pool;
+  const float* k_scales;  // [n_blocks, n_head_kv]
+  const float* v_scales;
+  const int* tables;    // [batch, max_blocks] (this layer)
+  const int* ctx_lens;  // [batch] (this layer)
+  const int* lens;      // [batch] or null
+  int64_t n_blocks;
+  int block_size, max_blocks, max_ctx, batch, seq_len, n_head, n_head_kv, head_dim;
+  int ctx_add, zero_to, causal;
+  float scale;
+  void* out;    // [batch, seq_len, n_head, head_dim]
+  float* part;  // paged_attn_workspace_floats
+};
+bool paged_attn_supported(int head_dim);
+size_t paged_attn_workspace_floats(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim,
+                                   int q_dtype);
+hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s);
+
 }  // namespace fmoe

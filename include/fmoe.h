@@ -82,7 +82,9 @@ const char *fmoe_last_error(void);
  *    fmoe_diag.h; FMOE_TIMER_QUANT added (FMOE_TIMER_COUNT 10 -> 11); dtype
  *    FMOE_F8E4M3FN_A8 (3); fmoe_moe_ffn_block_noalloc.  Packed-weight
  *    artifacts record the version they were written under.
- * 3: dtype FMOE_F8E4M3FN_A8X2 (4). */
+ * 3: dtype FMOE_F8E4M3FN_A8X2 (4).  The entry points on caches of e4m3 codes
+ *    came later under the same version: they changed no declaration that was
+ *    there, nor the packed layout. */
 int fmoe_abi_version(void);
 #define FMOE_ABI_VERSION 3
 
@@ -409,6 +411,78 @@ int fmoe_attention_sublayer_decode_paged(const void *residual, const void *attn_
                                          float rope_freq_base, float rope_freq_scale,
                                          int act_dtype, void *out, void *k_new, void *v_new,
                                          void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------- */
+/* A paged K/V cache in 8 bits, and attention of one or more new tokens.  No
+ * counterpart in the reference, whose cache holds fp32 and whose prefill
+ * attention runs on the new tokens alone (attention_block_prefill.mlir).
+ *
+ * A pool of codes: [n_blocks, block_size, n_head_kv, head_dim] FMOE_F8E4M3FN
+ * with scales [n_blocks, n_head_kv] float32; a value is code * scale of its
+ * (block, head).  head_dim is 16, 32, 64 or 128.
+ *
+ * fmoe_kvcache_append: the new tokens' keys (rotated at their positions,
+ * rope = 1) and values into the pages of block_tables [n_layers, batch,
+ * max_blocks_per_seq], and the queries, rotated, to q_out.
+ *   k, v [batch, seq_len, n_head_kv, head_dim], q [batch, seq_len, n_head,
+ *   head_dim] (null: none), all act_dtype (F32 or BF16); token (b, s) starts
+ *   (b * seq_len + s) * stride elements from the pointer (so the parts of one
+ *   fused projection row can be passed as they lie; strides of at least the
+ *   token's elements); pointers and stride * element size are multiples of
+ *   16 bytes.  q_out is laid out as q with a stride of its own; it may be q.
+ *   Token s of sequence b has position start_positions[b] + s; RoPE turns
+ *   the pairs (2i, 2i+1) by position * rope_freq_scale /
+ *   rope_freq_base^(2i/head_dim), angles in double precision.
+ *   seq_lens [batch] int32 (null: seq_len each): tokens at and past it are
+ *   padding, whose k and v are not read; their q is rotated like the others.
+ *   cache_dtype: act_dtype (k_scales, v_scales unused), or F8E4M3FN: an
+ *   append to rows [r0, r1) of a block with head-wise largest magnitude a
+ *   takes the least power of two s with a <= 448 s (2^-126 for a = 0) as the
+ *   block's scale if r0 = 0, and max(s, scale) otherwise; rows below r0 are
+ *   then rounded again to a grown scale.  What is not finite is stored as
+ *   NaN and left out of a.
+ *   An append ends its sequence: rows of the last block behind it keep their
+ *   codes, but stand for nothing.  Positions whose table entry lies outside
+ *   the pool, or past the table, are skipped.  When several blocks of one
+ *   call's tables name the same pool block, the last one (by sequence, then
+ *   position) alone is written. */
+int fmoe_kvcache_append(void *k_cache, void *v_cache, float *k_scales, float *v_scales,
+                        int cache_dtype, int64_t n_blocks, int64_t block_size, int64_t n_head_kv,
+                        int64_t head_dim, int64_t layer, const void *k, int64_t k_stride,
+                        const void *v, int64_t v_stride, const void *q, int64_t q_stride,
+                        void *q_out, int64_t q_out_stride, int64_t n_head, int act_dtype,
+                        int64_t batch, int64_t seq_len, const int32_t *block_tables,
+                        int64_t n_layers, int64_t max_blocks_per_seq,
+                        const int32_t *start_positions, const int32_t *seq_lens, int rope,
+                        float rope_freq_base, float rope_freq_scale, void *stream);
+
+/* Attention of the last seq_lens[b] (null: seq_len) tokens of each sequence's
+ * context over pools of codes (16-byte aligned):
+ *   q [batch, seq_len, n_head, head_dim] act_dtype (rotated; token stride
+ *   q_stride and alignment as above), out [batch, seq_len, n_head, head_dim]
+ *   contiguous, act_dtype; query head h reads K/V head h / (n_head / n_head_kv).
+ *   context_lens [n_layers, batch] int32 counts the cached positions, the new
+ *   tokens' own among them: token s of sequence b is position
+ *   context_lens[layer, b] - seq_lens[b] + s.  It attends the positions below
+ *   min(context_lens[layer, b], max_context_len), with causal = 1 only up to
+ *   its own.  score = q . K * scale (0: 1/sqrt(head_dim)), softmax in fp32.
+ * Tokens that attend nothing, and padding tokens (s >= seq_lens[b], whose q is
+ * not read), get zeros.  Table entries outside the pool or past the table are
+ * keys and values of zeros.  A position that a token does not attend has no
+ * influence on it, whatever its codes and scale hold.  Workspace:
+ * fmoe_attention_paged_workspace_bytes. */
+size_t fmoe_attention_paged_workspace_bytes(int64_t batch, int64_t seq_len,
+                                            int64_t max_context_len, int64_t n_head,
+                                            int64_t n_head_kv, int64_t head_dim, int act_dtype);
+int fmoe_attention_paged(const void *q, int64_t q_stride, const void *k_cache,
+                         const float *k_scales, const void *v_cache, const float *v_scales,
+                         int64_t n_blocks, int64_t block_size, int64_t layer,
+                         const int32_t *block_tables, const int32_t *context_lens,
+                         const int32_t *seq_lens, int64_t n_layers, int64_t batch,
+                         int64_t seq_len, int64_t max_blocks_per_seq, int64_t max_context_len,
+                         int64_t n_head, int64_t n_head_kv, int64_t head_dim, int causal,
+                         float scale, int act_dtype, void *out, void *workspace,
+                         size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
