@@ -1580,6 +1580,9 @@ int fmoe_attention_sublayer_decode_paged(const void* residual, const void* attn_
 }
 
 // ------------------------------------------------------------ caches of e4m3 codes
+// Positions are counted in 32 bits, a tile past the context's end included.
+static constexpr int64_t kMaxPagedContext = kMaxDim - 4096;
+
 // Shapes and pointers shared by the append and the attention over pages.
 static int check_pages(int64_t n_blocks, int64_t block_size, int64_t n_head_kv, int64_t head_dim, int64_t layer,
                        int64_t n_layers, int64_t batch, int64_t seq_len, int64_t max_blocks_per_seq) {
@@ -1672,7 +1675,7 @@ int fmoe_kvcache_append(void* k_cache, void* v_cache, float* k_scales, float* v_
 size_t fmoe_attention_paged_workspace_bytes(int64_t batch, int64_t seq_len, int64_t max_context_len, int64_t n_head,
                                             int64_t n_head_kv, int64_t head_dim, int act_dtype) {
   if (!act_dtype_ok(act_dtype) || batch < 0 || batch > 65535 || seq_len < 0 || seq_len > kMaxDim ||
-      max_context_len < 0 || max_context_len > kMaxDim || n_head_kv < 1 || n_head_kv > n_head || n_head > 65535 ||
+      max_context_len < 0 || max_context_len > kMaxPagedContext || n_head_kv < 1 || n_head_kv > n_head || n_head > 65535 ||
       n_head % n_head_kv || !paged_attn_supported(static_cast<int>(std::min<int64_t>(head_dim, kMaxDim))))
     return 0;
   return align_up(paged_attn_workspace_floats(static_cast<int>(batch), static_cast<int>(seq_len),
@@ -1693,7 +1696,7 @@ int fmoe_attention_paged(const void* q, int64_t q_stride, const void* k_cache, c
                        max_blocks_per_seq));
   FMOE_TRY(check_dims("n_head", n_head, n_head_kv, 65535));
   if (n_head % n_head_kv) return fail(FMOE_ERR_SHAPE, "n_head %% n_head_kv != 0");
-  FMOE_TRY(check_dims("max_context_len", max_context_len, 0, kMaxDim));
+  FMOE_TRY(check_dims("max_context_len", max_context_len, 0, kMaxPagedContext));
   if (seq_len > 0) FMOE_TRY(check_dims("seq_len * n_head", seq_len, 0, kMaxDim / n_head));
   if (causal != 0 && causal != 1) return fail(FMOE_ERR_INVALID_ARGUMENT, "causal must be 0 or 1");
   if (!(scale >= 0.f && std::isfinite(scale)))

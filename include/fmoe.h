@@ -466,6 +466,7 @@ int fmoe_kvcache_append(void *k_cache, void *v_cache, float *k_scales, float *v_
  *   context_lens[layer, b] - seq_lens[b] + s.  It attends the positions below
  *   min(context_lens[layer, b], max_context_len), with causal = 1 only up to
  *   its own.  score = q . K * scale (0: 1/sqrt(head_dim)), softmax in fp32.
+ *   max_context_len is at most 2^31 - 4097.
  * Tokens that attend nothing, and padding tokens (s >= seq_lens[b], whose q is
  * not read), get zeros.  Table entries outside the pool or past the table are
  * keys and values of zeros.  A position that a token does not attend has no
