@@ -86,6 +86,9 @@ __device__ __forceinline__ int limit_of(const PagedAttnArgs& a, const Span& s, i
   return a.causal ? static_cast<int>(min(max(s.pos + t + 1, int64_t{0}), static_cast<int64_t>(s.cut))) : s.cut;
 }
 
+// The n lowest bits.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0ull; }
+
 __device__ __forceinline__ void store_out(const PagedAttnArgs& a, int64_t i, float v) {
   if (a.out_dtype == DT_F32)
     static_cast<float*>(a.out)[i] = v;
@@ -297,11 +300,18 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
       zero_now[h] = zero[h];
     }
     const bool full = (valid_now[0] & valid_now[1]) == ~0ull && at + kChunk <= first_limit;
-    // Whether this lane's row attends position 16 st + 4 q4 + i of the chunk,
-    // a row of the pool.
-    auto attends = [&](int st, int i) __attribute__((always_inline)) {
-      return (valid_now[st / 4] >> (16 * (st % 4) + 4 * q4 + i) & 1) && at + 16 * st + 4 * q4 + i < limit;
-    };
+    // Positions that this lane's row attends: rows of the pool, and rows of
+    // zeros; bit 16 (st % 4) + i of word st / 4 belongs to score i of sc[st].
+    uint64_t on[2] = {~0ull, ~0ull}, nil[2] = {0ull, 0ull};
+    if (!full) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t below = low_bits(limit - at - 64 * h);
+        on[h] = (valid_now[h] & below) >> (4 * q4);
+        nil[h] = (zero_now[h] & below) >> (4 * q4);
+      }
+    }
+    auto attends = [&](int st, int i) __attribute__((always_inline)) { return (on[st / 4] >> (16 * (st % 4) + i) & 1) != 0; };
     load_table(min(c + 1, n - 1));  // always two loads, so that the waits below count alike
 
     // ---- scores.  In flight behind K tile `it`: the tiles after it (K,
@@ -348,10 +358,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[i] *= kscale[u][i];
         if (!full) {
-          const uint64_t zm = zero_now[st / 4] >> (16 * (st % 4) + 4 * q4);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            d[i] = attends(st, i) ? d[i] : zm >> i & 1 && at + 16 * st + 4 * q4 + i < limit ? 0.f : -INFINITY;
+            d[i] = attends(st, i) ? d[i] : nil[st / 4] >> (16 * (st % 4) + i) & 1 ? 0.f : -INFINITY;
         }
         sc[st] = d;
       }
@@ -451,11 +460,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
         }
         if (__builtin_expect(bad, 0)) {
           // 1 where this lane's row attends the position
-          float on[8];
+          float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) on[e] = attends(2 * pg + e / 4, e % 4) ? 1.f : 0.f;
+          for (int e = 0; e < 8; ++e) y[e] = attends(2 * pg + e / 4, e % 4) ? 1.f : 0.f;
           u32x4_t one[1];
-          split8<1>(on, one);
+          split8<1>(y, one);
 #pragma unroll
           for (int t = 0; t < D / 16; ++t) {
             const uint32_t n0 = (nan_bytes(w[g][t][0]) >> 7) * 0xFFu, n1 = (nan_bytes(w[g][t][1]) >> 7) * 0xFFu;
@@ -517,6 +526,391 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   }
 }
 
+// ------------------------------------------------------------------ many rows
+// Block (row tile of 128, K/V head, context split; sequence): wave w has 32
+// rows, and the four share tiles of 64 positions, three in LDS: while one is
+// computed the next two are in flight (global_load_lds; one block barrier a
+// tile).  Bound by the matrix cores and, beside them, by the vector work of
+// the softmax; 64 positions of 32 rows are 1024 cycles of products at
+// head_dim 128 and about as many of vector instructions.
+// Scores: v_mfma_scale_f32_32x32x64_f8f6f4 with A = the K codes as they lie
+// and B = q as two e4m3 terms under a power of two of the row: hi = e4m3(q/s),
+// lo = e4m3(q/s - hi), exact for bf16 values down to s/4 and within s/1024
+// below.  Two fp8 products cost what one bf16 product does and spare the
+// conversion of K.  A lane holds, for row l % 32, positions 8 i + 4 (l / 32)
+// + 0..3, which serve as the B operand of the second product in bf16
+// (32x32x16) with A = V transposed, converted as it is read.
+// The running maximum is raised, and the sums rescaled, only when a row's
+// has grown by more than 2^kLazy: weights are then at most 2^kLazy, which fp32
+// sums and bf16 operands hold as well.
+constexpr int kBigRows = 128;
+constexpr int kWaveRows = 32;
+constexpr int kBigTile = 64;
+constexpr int kStages = 3;
+constexpr float kLazy = 8.f;
+
+typedef __attribute__((ext_vector_type(8))) int i32x8_t;
+
+__device__ __forceinline__ f32x16_t mfma32(const u32x4_t a, const u32x4_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16_t mfma32_f8(const i32x8_t a, const i32x8_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+// Maximum of lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int D>
+struct Big {
+  static constexpr int kPieces = D / 16;
+  static constexpr int kRowsPerLoad = 1024 / D;
+  static constexpr int kLoads = kBigTile / kRowsPerLoad / kWaves;  // of K, and of V, per wave and tile
+  static constexpr int kTileB = kBigTile * D;
+  static constexpr int kScaleB = kWaves * kWave * 4;
+  static constexpr int kStageB = 2 * kTileB + kScaleB;
+  static constexpr int kLds = kStages * kStageB + kStages * kWaves * 4;
+  static constexpr int kPerTile = 2 * kLoads + 1;  // loads per wave and tile
+  static constexpr int kWaveTileRows = kBigTile / kWaves;
+  static_assert(kLoads * kRowsPerLoad == kWaveTileRows, "a wave loads whole rows");
+};
+
+// As v_place, for the rows that one read of 32 columns touches: bits 0, 1 and
+// 3 vary, and the piece's lowest bit.
+template <int D>
+__device__ __forceinline__ int v_place32(int r) {
+  return D == 128 ? ((r >> 1) & 1) << 1 | ((r >> 3) & 1) << 2 : ((r >> 3) & 1) << 1;
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a, int n_split, int split_len) {
+  using R = Big<D>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  uint32_t* flags = reinterpret_cast<uint32_t*>(lds + kStages * R::kStageB);  // [stage][wave]: valid, zero << 16
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int half = lane >> 5, col = lane & 31;
+  const int G = a.n_head / a.n_head_kv;
+  const int b = blockIdx.y;
+  const int split = blockIdx.x % n_split, kvh = blockIdx.x / n_split % a.n_head_kv;
+  // the tiles of the last tokens, which attend most, go first
+  const int n_tiles = gridDim.x / n_split / a.n_head_kv;
+  const int row0 = (n_tiles - 1 - static_cast<int>(blockIdx.x / n_split / a.n_head_kv)) * kBigRows;
+  const Span span = span_of(a, b);
+
+  const int wave_row0 = row0 + wave * kWaveRows;
+  const int token = (wave_row0 + col) / G, head = kvh * G + (wave_row0 + col) % G;
+  const int limit = limit_of(a, span, token);
+  auto end_of = [&](int first, int n) {  // positions that rows [first, first + n) attend
+    return first / G < span.len ? limit_of(a, span, min((first + n - 1) / G, span.len - 1)) : 0;
+  };
+  const int j0 = split * split_len;
+  const int end = min(end_of(row0, kBigRows), j0 + split_len);  // of this block
+  const int wave_end = min(end_of(wave_row0, kWaveRows), j0 + split_len);
+  const int first_limit = limit_of(a, span, wave_row0 / G);
+  const int n = end > j0 ? (end - j0 + kBigTile - 1) / kBigTile : 0;
+  if (n == 0 && n_split > 1) return;  // the combine reads only the splits with positions
+
+  const int* seq_table = a.tables + static_cast<int64_t>(b) * a.max_blocks;
+  const int64_t row_b = static_cast<int64_t>(a.n_head_kv) * D;
+  const uint8_t* kp = a.k_pool + kvh * D;
+  const uint8_t* vp = a.v_pool + kvh * D;
+
+  // ---- loads.  Lanes l and l % 16 stand for position 16 wave + l % 16 of a tile.
+  const int wp = wave * R::kWaveTileRows + (lane & 15);
+  int next_page = (j0 + wp) / a.block_size, next_off = (j0 + wp) % a.block_size;
+  const int page_step = kBigTile / a.block_size, off_step = kBigTile % a.block_size;
+  int entry = 0;  // table entry of the tile that load_tile takes next
+  auto load_entry = [&]() __attribute__((always_inline)) { entry = seq_table[min(next_page, a.max_blocks - 1)]; };
+  const int lr = lane / R::kPieces, lc = lane % R::kPieces;
+  int next_j = j0 + wp;
+  auto load_tile = [&](int stage) __attribute__((always_inline)) {
+    const bool in = next_j < end, ok = next_page < a.max_blocks && entry >= 0 && entry < a.n_blocks;
+    const int row = in && ok ? entry * a.block_size + next_off : -1;
+    const uint32_t valid = static_cast<uint32_t>(__ballot(row >= 0)) & 0xFFFFu;
+    const uint32_t zero = static_cast<uint32_t>(__ballot(in && !ok)) & 0xFFFFu;
+    // unusable rows load a usable one
+    const int first = valid ? __builtin_amdgcn_readlane(row, __builtin_ctz(valid)) : 0;
+    const int use = row >= 0 ? row : first;
+    const int page = row >= 0 ? entry : first / a.block_size;
+    unsigned char* base = lds + stage * R::kStageB;
+    if (lane == 0) flags[stage * kWaves + wave] = valid | zero << 16;
+    int r[R::kLoads];
+#pragma unroll
+    for (int i = 0; i < R::kLoads; ++i) r[i] = __shfl(use, i * R::kRowsPerLoad + lr, kWave);
+    next_j += kBigTile;
+    next_page += page_step;
+    next_off += off_step;
+    if (next_off >= a.block_size) {
+      next_off -= a.block_size;
+      ++next_page;
+    }
+    load_entry();  // before the tile's own loads, which a wait for it leaves in flight
+    const float* scales = lane & 16 ? a.v_scales : a.k_scales;
+    load_lds4(scales + static_cast<int64_t>(page) * a.n_head_kv + kvh, base + 2 * R::kTileB + wave * kWave * 4);
+#pragma unroll
+    for (int i = 0; i < R::kLoads; ++i) {
+      const int tr = wave * R::kWaveTileRows + i * R::kRowsPerLoad + lr;
+      const int at = (wave * R::kLoads + i) * 1024;
+      load_lds16(kp + r[i] * row_b + ((lc ^ k_place<D>(tr)) << 4), base + at);
+      load_lds16(vp + r[i] * row_b + ((lc ^ v_place32<D>(tr)) << 4), base + R::kTileB + at);
+    }
+  };
+
+  // ---- q as two terms: lane (half, col) holds dimensions 64 s + 32 half + 0..31 of row col
+  i32x8_t qh[D / 64], ql[D / 64];
+  float c2, q_scale;
+  {
+    const int64_t at = (static_cast<int64_t>(b) * a.seq_len + token) * a.q_stride + static_cast<int64_t>(head) * D;
+    u32x4_t w[D / 64][4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[s][i] = u32x4_t{0u, 0u, 0u, 0u};
+        if (token < span.len)
+          w[s][i] = *reinterpret_cast<const u32x4_t*>(static_cast<const bf16_t*>(a.q) + at + 64 * s + 32 * half + 8 * i);
+      }
+#pragma unroll
+    for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max(w[s][i][e] << 16 & 0x7FFFFFFFu, w[s][i][e] & 0x7FFF0000u));
+    top = __float_as_uint(max_halves(__uint_as_float(min(top, 0x7F800000u))));
+    float inv = 1.f;
+    q_scale = pow2_scale(__uint_as_float(min(top, 0x7F7F0000u)), &inv);
+#pragma unroll
+    for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x2_t hi, lo;
+        e4m3_codes8_x2(w[s][i], inv, hi, lo);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          qh[s][2 * i + e] = static_cast<int>(hi[e]);
+          ql[s][2 * i + e] = static_cast<int>(lo[e]);
+        }
+      }
+    // a row that is not finite has scores that are NaN
+    c2 = top >= 0x7F800000u ? __builtin_nanf("") : a.scale * kLog2e * q_scale;
+#pragma unroll
+    for (int s = 0; s < D / 64; ++s) asm volatile("" : "+v"(qh[s]), "+v"(ql[s]));  // loaded here, not between the tiles
+  }
+
+  float m = -INFINITY, l = 0.f;
+  f32x16_t acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+
+  if (n > 0) {
+    load_entry();
+    load_tile(0);
+    load_tile(1);  // past the end: rows that are not used
+  }
+  int stage = 0;
+  for (int t = 0; t < n; ++t) {
+    // This wave's part of tile t is there (behind it: the next tile's loads
+    // and its table entry), and so is everyone's after the barrier, which no
+    // wave passes before all have read tile t - 1: its stage is free.
+    __builtin_amdgcn_s_waitcnt(wait_vm(R::kPerTile + 1, true));
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    load_tile(stage >= 1 ? stage - 1 : kStages - 1);
+    const unsigned char* base = lds + stage * R::kStageB;
+    const float* scales = reinterpret_cast<const float*>(base + 2 * R::kTileB);
+    const u32x4_t fl = *reinterpret_cast<const u32x4_t*>(flags + stage * kWaves);
+    stage = stage + 1 < kStages ? stage + 1 : 0;
+    const int at = j0 + t * kBigTile;
+    if (at >= wave_end) continue;  // none of this wave's rows
+    const uint64_t lo16 = (fl[0] & 0xFFFFu) | fl[1] << 16, hi16 = (fl[2] & 0xFFFFu) | fl[3] << 16;
+    const uint64_t valid = lo16 | hi16 << 32;
+    const uint64_t zero = static_cast<uint64_t>((fl[0] >> 16) | (fl[1] & 0xFFFF0000u)) |
+                          static_cast<uint64_t>((fl[2] >> 16) | (fl[3] & 0xFFFF0000u)) << 32;
+    const bool full = __builtin_amdgcn_readfirstlane(static_cast<int>(valid == ~0ull)) && at + kBigTile <= first_limit;
+    // Positions that this lane's row attends: rows of the pool, and rows of
+    // zeros; bit 32 pt + 8 (i / 4) + i % 4 belongs to score i of sc[pt].
+    uint32_t on[2] = {~0u, ~0u}, nil[2] = {0u, 0u};
+    if (!full) {
+      const uint64_t below = low_bits(limit - at);
+      const uint64_t o = (valid & below) >> (4 * half), z = (zero & below) >> (4 * half);
+      on[0] = static_cast<uint32_t>(o);
+      on[1] = static_cast<uint32_t>(o >> 32);
+      nil[0] = static_cast<uint32_t>(z);
+      nil[1] = static_cast<uint32_t>(z >> 32);
+    }
+
+    // ---- scores
+    f32x16_t sc[2];
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[pt][i] = 0.f;
+      const int r = 32 * pt + col;
+#pragma unroll
+      for (int s = 0; s < D / 64; ++s) {
+        u32x4_t w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          w[e] = *reinterpret_cast<const u32x4_t*>(base + r * D + (((4 * s + 2 * half + e) ^ k_place<D>(r)) << 4));
+        const i32x8_t k = __builtin_bit_cast(i32x8_t, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        sc[pt] = mfma32_f8(k, qh[s], sc[pt]);
+        sc[pt] = mfma32_f8(k, ql[s], sc[pt]);
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t ks = *reinterpret_cast<const f32x4_t*>(scales + (2 * pt + g / 2) * kWave + 8 * (g % 2) + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[pt][4 * g + i] *= ks[i];
+      }
+    if (!full) {
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t bit = 1u << (8 * (i >> 2) + (i & 3));
+          sc[pt][i] = on[pt] & bit ? sc[pt][i] : nil[pt] & bit ? 0.f : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[pt][i]);
+    mx = max_halves(mx);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- softmax
+    if (__any((mx - m) * c2 > kLazy)) {
+      const float top = fmaxf(m, mx);
+      const float f = __builtin_amdgcn_exp2f((m - finite_base(top)) * c2);
+      m = top;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+    }
+    const float mc = finite_base(m) * c2;
+    u32x4_t p[4];
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt) {
+      float w[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t vs =
+            *reinterpret_cast<const f32x4_t*>(scales + (2 * pt + g / 2) * kWave + 16 + 8 * (g % 2) + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(sc[pt][4 * g + i], c2, -mc));
+          l += e;
+          w[4 * g + i] = e * vs[i];
+        }
+      }
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(on[pt] & 1u << (8 * (i >> 2) + (i & 3)))) w[i] = 0.f;  // 0 times a scale that is not finite
+      }
+      split8<1>(w, &p[2 * pt]);
+      split8<1>(w + 8, &p[2 * pt + 1]);
+    }
+
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- values
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = (lane & 15) >> 1, r = 16 * s + 8 * (k >> 2) + 4 * half + (k & 3);
+      const unsigned char* row = base + R::kTileB + r * D + 8 * (lane & 1);
+      u32x2_t w[D / 32];
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+        w[d] = read_columns(row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4));
+      if (!full) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) any |= nan_bytes(w[d][0]) | nan_bytes(w[d][1]);
+        if (__builtin_expect(__any(any != 0), 0)) {
+          float y[8];  // 1 where this lane's row attends the position
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = on[s / 2] & 1u << (8 * (2 * (s % 2) + e / 4) + e % 4) ? 1.f : 0.f;
+          u32x4_t one[1];
+          split8<1>(y, one);
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) {
+            const uint32_t n0 = (nan_bytes(w[d][0]) >> 7) * 0xFFu, n1 = (nan_bytes(w[d][1]) >> 7) * 0xFFu;
+            w[d][0] &= ~n0;
+            w[d][1] &= ~n1;
+            f32x16_t hit;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) hit[i] = 0.f;
+            hit = mfma32(f8x8_to_bf16x8(n0 & 0x38383838u, n1 & 0x38383838u), one[0], hit);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (hit[i] > 0.f) acc[d][i] = __builtin_nanf("");
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) acc[d] = mfma32(f8x8_to_bf16x8(w[d][0], w[d][1]), p[s], acc[d]);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm(0, true));  // the loads past the end
+
+  // ---- this wave's rows: lane (half, col) holds dimensions 32 d + 8 i + 4 half + 0..3 of row col
+  l = sum_halves(l);
+  if (token >= a.seq_len) return;
+  const int64_t row = (static_cast<int64_t>(b) * a.seq_len + token) * a.n_head + head;
+  const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
+  if (n_split == 1) {
+    const int zeros = token < span.len ? max(a.zero_to - span.cut, 0) : 0;
+    float f = 1.f;
+    if (zeros > 0) {
+      const float top = fmaxf(m, 0.f);
+      f = __builtin_amdgcn_exp2f((m - top) * c2);
+      l = fmaf(l, f, static_cast<float>(zeros) * __builtin_amdgcn_exp2f(-top * c2));
+    }
+    f = token >= span.len || l == 0.f ? 0.f : f / l;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const u32x2_t w{pack_bf16x2(acc[d][4 * g] * f, acc[d][4 * g + 1] * f),
+                        pack_bf16x2(acc[d][4 * g + 2] * f, acc[d][4 * g + 3] * f)};
+        *reinterpret_cast<u32x2_t*>(static_cast<bf16_t*>(a.out) + row * D + 32 * d + 8 * g + 4 * half) =
+            token >= span.len ? u32x2_t{0u, 0u} : w;
+      }
+  } else if (limit > j0) {
+    float* part = a.part + (row * n_split + split) * D;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4_t*>(part + 32 * d + 8 * g + 4 * half) =
+            f32x4_t{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+    if (half == 0)
+      *reinterpret_cast<float2*>(a.part + n_rows * n_split * D + (row * n_split + split) * 2) = float2{m * q_scale, l};
+  }
+}
+
 // ------------------------------------------------------------------ joining the splits
 // One wave per output row: the splits that hold positions of it, in order.
 constexpr int kJoinUnroll = 8;
@@ -569,21 +963,43 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
   }
 }
 
-// How the context is cut: splits of split_len positions, for two blocks per
-// CU where the rows alone do not give them.
+// Which kernel, and how the context is cut: splits of split_len positions,
+// for two blocks per CU where the rows alone do not give them.
 struct Plan {
+  bool big;
   int n_split, split_len;
 };
 
-Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv) {
+constexpr int kBigFrom = 64;  // query rows of a K/V head
+
+Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int q_dtype) {
   const int64_t rows = static_cast<int64_t>(seq_len) * (n_head / n_head_kv);
-  const int64_t blocks = static_cast<int64_t>(batch) * n_head_kv * ((rows + kRows - 1) / kRows);
+  Plan p;
+  p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom;
+  const int tile = p.big ? kBigRows : kRows, step = p.big ? 4 * kBigTile : 2 * kChunk;
+  const int64_t blocks = static_cast<int64_t>(batch) * n_head_kv * ((rows + tile - 1) / tile);
   int64_t n = blocks > 0 ? (512 + blocks - 1) / blocks : 1;
   int64_t len = (max_ctx + n - 1) / n;
-  len = (len + 2 * kChunk - 1) / (2 * kChunk) * (2 * kChunk);  // no shorter than two waves' chunks
-  if (len < 2 * kChunk) len = 2 * kChunk;
+  len = (len + step - 1) / step * step;
+  if (len < step) len = step;
   n = (max_ctx + len - 1) / len;
-  return Plan{static_cast<int>(n < 1 ? 1 : n), static_cast<int>(len)};
+  p.n_split = static_cast<int>(n < 1 ? 1 : n);
+  p.split_len = static_cast<int>(len);
+  return p;
+}
+
+template <int D>
+void launch_big(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
+  if constexpr (D >= 64) {
+    constexpr int lds = Big<D>::kLds;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_tile_kernel<D>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    (void)attr;
+    const int64_t rows = static_cast<int64_t>(a.seq_len) * (a.n_head / a.n_head_kv);
+    const int64_t x = (rows + kBigRows - 1) / kBigRows * a.n_head_kv * p.n_split;
+    hipLaunchKernelGGL((paged_tile_kernel<D>), dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), lds, s, a,
+                       p.n_split, p.split_len);
+  }
 }
 
 template <int D, int kTerms>
@@ -600,8 +1016,10 @@ void launch_stream(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
 
 template <int D>
 hipError_t launch_dim(const PagedAttnArgs& a, hipStream_t s) {
-  const Plan p = plan_of(a.batch, a.seq_len, a.max_ctx, a.n_head, a.n_head_kv);
-  if (a.q_dtype == DT_F32)
+  const Plan p = plan_of(a.batch, a.seq_len, a.max_ctx, a.n_head, a.n_head_kv, D, a.q_dtype);
+  if (p.big)
+    launch_big<D>(a, p, s);
+  else if (a.q_dtype == DT_F32)
     launch_stream<D, 3>(a, p, s);
   else
     launch_stream<D, 1>(a, p, s);
@@ -619,8 +1037,9 @@ bool paged_attn_supported(int head_dim) {
   return head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128;
 }
 
-size_t paged_attn_workspace_floats(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int) {
-  const Plan p = plan_of(batch, seq_len, max_ctx, n_head, n_head_kv);
+size_t paged_attn_workspace_floats(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim,
+                                   int q_dtype) {
+  const Plan p = plan_of(batch, seq_len, max_ctx, n_head, n_head_kv, head_dim, q_dtype);
   if (p.n_split <= 1) return 0;
   return static_cast<size_t>(batch) * seq_len * n_head * p.n_split * (head_dim + 2);
 }
