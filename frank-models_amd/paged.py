@@ -14,13 +14,29 @@ comes back as NumPy.  Pools are device tensors, updated in place.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib as L
-from .api import _TORCH_TO_DT, _device, _finish, _ptr, _stream, _to_device, _workspace
+from .api import _TORCH_TO_DT, _device, _finish, _to_device
 from .attention import _ints_to_device
+
+# A decode step makes a call of each per layer, whose kernels take a few
+# microseconds: the checks ask tensors for plain numbers (device index, shape,
+# strides) and leave what is in order as it is.
+
+
+def _here() -> int:
+    """The current device's index."""
+    if not torch.cuda.is_initialized():
+        _device()  # NoDeviceError where there is none
+    return torch.cuda.current_device()
+
+
+def _raw_stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 @dataclass
@@ -48,68 +64,93 @@ class QuantizedKVPool:
         return self.data.view(torch.float8_e4m3fn).float() * self.scales[:, None, :, None]
 
 
+_CODES = (torch.float8_e4m3fn, torch.uint8)
+
+
 def _check_pool(pool, name, dev):
-    """-> (data, scales or None) of a pool argument, checked."""
-    data, scales = (pool.data, pool.scales) if isinstance(pool, QuantizedKVPool) else (pool, None)
-    if not isinstance(data, torch.Tensor) or data.device != dev or not data.is_contiguous():
-        raise TypeError(f"{name} must be a contiguous tensor on {dev}")
-    if data.dim() != 4:
-        raise ValueError(f"{name} must be [n_blocks, block_size, n_head_kv, head_dim], got {tuple(data.shape)}")
-    if isinstance(pool, QuantizedKVPool):
-        if data.dtype not in (torch.float8_e4m3fn, torch.uint8):
+    """-> (data, scales or None, shape) of a pool argument, checked."""
+    quantized = isinstance(pool, QuantizedKVPool)
+    data, scales = (pool.data, pool.scales) if quantized else (pool, None)
+    if not isinstance(data, torch.Tensor) or data.get_device() != dev or not data.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous tensor on the current device, cuda:{dev}")
+    shape = data.shape
+    if len(shape) != 4:
+        raise ValueError(f"{name} must be [n_blocks, block_size, n_head_kv, head_dim], got {tuple(shape)}")
+    if quantized:
+        if data.dtype not in _CODES:
             raise TypeError(f"{name}: codes must be float8_e4m3fn or uint8, got {data.dtype}")
-        if (not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or scales.device != dev
+        if (not isinstance(scales, torch.Tensor) or scales.dtype is not torch.float32 or scales.get_device() != dev
                 or not scales.is_contiguous()):
-            raise TypeError(f"{name}: scales must be a contiguous float32 tensor on {dev}")
-        if scales.shape != (data.shape[0], data.shape[2]):
-            raise ValueError(f"{name}: scales must be [n_blocks, n_head_kv] = [{data.shape[0]}, {data.shape[2]}]")
-    return data, scales
+            raise TypeError(f"{name}: scales must be a contiguous float32 tensor on the current device, cuda:{dev}")
+        if scales.shape != (shape[0], shape[2]):
+            raise ValueError(f"{name}: scales must be [n_blocks, n_head_kv] = [{shape[0]}, {shape[2]}]")
+    return data, scales, shape
 
 
 def _check_pools(k_cache, v_cache, dev):
-    k, ks = _check_pool(k_cache, "k_cache", dev)
-    v, vs = _check_pool(v_cache, "v_cache", dev)
-    if k.shape != v.shape or (ks is None) != (vs is None) or (ks is None and k.dtype != v.dtype):
-        raise ValueError(f"k_cache {tuple(k.shape)} and v_cache {tuple(v.shape)} must have one shape and type")
-    if k.data_ptr() == v.data_ptr():
+    k, ks, shape = _check_pool(k_cache, "k_cache", dev)
+    v, vs, v_shape = _check_pool(v_cache, "v_cache", dev)
+    if shape != v_shape or (ks is None) != (vs is None) or (ks is None and k.dtype is not v.dtype):
+        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v_shape)} must have one shape and type")
+    if k.data_ptr() == v.data_ptr() and k.numel():
         raise ValueError("k_cache and v_cache must be two pools")
-    return k, ks, v, vs
+    return k, ks, v, vs, shape
 
 
 def _tokens(x, name, heads, dim, dev):
     """A [batch, seq_len, heads, dim] operand -> (tensor, elements between
-    tokens, came from NumPy).  Views whose tokens lie at one stride, as the
-    parts of a fused projection row do, are read in place; others are copied."""
-    x, from_np = (x, False) if isinstance(x, torch.Tensor) and x.dtype in _TORCH_TO_DT and x.is_cuda else _to_device(x, name)
-    if x.device != dev:
-        raise ValueError(f"{name} must be on the current device {dev}, got {x.device}")
-    if x.dim() != 4 or x.shape[3] != dim or (heads is not None and x.shape[2] != heads):
+    tokens, shape, came from NumPy).  Views whose tokens lie at one stride, as
+    the parts of a fused projection row do, are read in place; others are
+    copied."""
+    from_np = False
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _TORCH_TO_DT):
+        x, from_np = _to_device(x, name)
+    if x.get_device() != dev:
+        raise ValueError(f"{name} must be on the current device, cuda:{dev}, got {x.device}")
+    shape = x.shape
+    if len(shape) != 4 or shape[3] != dim or (heads is not None and shape[2] != heads):
         want = f"[batch, seq_len, {'n_head' if heads is None else heads}, {dim}]"
-        raise ValueError(f"{name} must be {want}, got {tuple(x.shape)}")
-    B, S, H, _ = x.shape
+        raise ValueError(f"{name} must be {want}, got {tuple(shape)}")
+    B, S, H, _ = shape
     sb, ss, sh, sd = x.stride()
     token = ss if S > 1 else sb if B > 1 else H * dim
-    if not ((sd == 1) and (sh == dim or H == 1) and (S == 1 or B == 1 or sb == S * ss) and token >= H * dim
+    if not (sd == 1 and (sh == dim or H == 1) and (S == 1 or B == 1 or sb == S * ss) and token >= H * dim
             and token * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0):
-        x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+        x = torch.empty(shape, dtype=x.dtype, device=x.device).copy_(x)
         token = H * dim
-    return x, token, from_np
+    return x, token, shape, from_np
 
 
-def _check_tables(block_tables, batch):
-    bt = _ints_to_device(block_tables, "block_tables")
-    if bt.dim() != 3 or bt.shape[1] != batch:
-        raise ValueError(f"block_tables must be [n_layers, {batch}, max_blocks], got {tuple(bt.shape)}")
-    return bt
+def _ints(a, name):
+    if type(a) is torch.Tensor and a.dtype is torch.int32 and a.is_cuda and a.is_contiguous():
+        return a
+    return _ints_to_device(a, name)
 
 
-def _per_sequence(a, name, batch):
-    if a is None:
-        return None
-    t = _ints_to_device(a, name)
+def _check_tables(block_tables, batch, dev):
+    """-> (block_tables, n_layers, max_blocks)."""
+    bt = _ints(block_tables, "block_tables")
+    shape = bt.shape
+    if len(shape) != 3 or shape[1] != batch:
+        raise ValueError(f"block_tables must be [n_layers, {batch}, max_blocks], got {tuple(shape)}")
+    if bt.get_device() != dev:
+        raise ValueError(f"block_tables must be on the current device, cuda:{dev}")
+    return bt, shape[0], shape[2]
+
+
+def _per_sequence(a, name, batch, dev):
+    t = _ints(a, name)
     if t.shape != (batch,):
         raise ValueError(f"{name} must be [{batch}], got {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on the current device, cuda:{dev}")
     return t
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch, seq_len, max_context_len, n_head, n_head_kv, head_dim, dt):
+    return L.lib().fmoe_attention_paged_workspace_bytes(batch, seq_len, max_context_len, n_head, n_head_kv, head_dim,
+                                                        dt)
 
 
 def kvcache_append(k_cache, v_cache, layer: int, k, v, block_tables, start_positions, *, seq_lens=None, q=None,
@@ -132,46 +173,45 @@ def kvcache_append(k_cache, v_cache, layer: int, k, v, block_tables, start_posit
     nothing.  Positions without a block in the pool are skipped; a block
     that the call's tables name several times is written by the last
     sequence and position alone."""
-    dev = _device()
-    kc, ks, vc, vs = _check_pools(k_cache, v_cache, dev)
-    n_blocks, bs, hkv, d = kc.shape
-    k, k_stride, _ = _tokens(k, "k", hkv, d, dev)
-    v, v_stride, _ = _tokens(v, "v", hkv, d, dev)
-    if k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must agree")
-    if ks is None and kc.dtype != k.dtype:
-        raise TypeError(f"a {kc.dtype} pool takes {kc.dtype} keys and values, got {k.dtype}")
-    batch, seq_len = k.shape[:2]
-    bt = _check_tables(block_tables, batch)
-    start = _per_sequence(start_positions, "start_positions", batch)
-    if start is None:
-        raise ValueError("start_positions must be [batch]")
-    lens = _per_sequence(seq_lens, "seq_lens", batch)
-    n_head, q_stride, out_stride, from_np, q_out_copy = 1, 0, 0, False, None
+    dev = _here()
+    kc, ks, vc, vs, (n_blocks, bs, hkv, d) = _check_pools(k_cache, v_cache, dev)
+    k, k_stride, shape, _ = _tokens(k, "k", hkv, d, dev)
+    v, v_stride, v_shape, _ = _tokens(v, "v", hkv, d, dev)
+    dtype = k.dtype
+    if shape != v_shape or dtype is not v.dtype:
+        raise ValueError(f"k {tuple(shape)} {dtype} and v {tuple(v_shape)} {v.dtype} must agree")
+    if ks is None and kc.dtype is not dtype:
+        raise TypeError(f"a {kc.dtype} pool takes {kc.dtype} keys and values, got {dtype}")
+    batch, seq_len = shape[0], shape[1]
+    bt, n_layers, max_blocks = _check_tables(block_tables, batch, dev)
+    start = _per_sequence(start_positions, "start_positions", batch, dev)
+    lens = None if seq_lens is None else _per_sequence(seq_lens, "seq_lens", batch, dev)
+    n_head, q_stride, out, out_stride, from_np = 1, 0, None, 0, False
     if q is not None:
-        q, q_stride, from_np = _tokens(q, "q", None, d, dev)
-        if q.dtype != k.dtype or q.shape[:2] != k.shape[:2]:
-            raise ValueError(f"q {tuple(q.shape)} {q.dtype} does not go with k {tuple(k.shape)} {k.dtype}")
-        n_head = q.shape[2]
+        q, q_stride, q_shape, from_np = _tokens(q, "q", None, d, dev)
+        if q.dtype is not dtype or q_shape[0] != batch or q_shape[1] != seq_len:
+            raise ValueError(f"q {tuple(q_shape)} {q.dtype} does not go with k {tuple(shape)} {dtype}")
+        n_head = q_shape[2]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        if not isinstance(q_out, torch.Tensor) or q_out.dtype != q.dtype or q_out.shape != q.shape \
-                or q_out.device != dev:
-            raise ValueError(f"q_out must be a {q.dtype} tensor {tuple(q.shape)} on {dev}")
-        out, out_stride, _ = _tokens(q_out, "q_out", n_head, d, dev)
-        if out is not q_out:
-            q_out_copy, q_out = q_out, out
+            q_out = out = q.new_empty(q_shape)
+            out_stride = n_head * d
+        elif (not isinstance(q_out, torch.Tensor) or q_out.dtype is not dtype or q_out.shape != q_shape
+              or q_out.get_device() != dev):
+            raise ValueError(f"q_out must be a {dtype} tensor {tuple(q_shape)} on cuda:{dev}")
+        else:
+            out, out_stride, _, _ = _tokens(q_out, "q_out", n_head, d, dev)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    L.call("fmoe_kvcache_append", _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs),
-           _TORCH_TO_DT[kc.dtype] if ks is None else L.F8E4M3FN, n_blocks, bs, hkv, d, int(layer), _ptr(k), k_stride,
-           _ptr(v), v_stride, _ptr(q), q_stride, _ptr(q_out), out_stride, n_head, _TORCH_TO_DT[k.dtype], batch,
-           seq_len, _ptr(bt), bt.shape[0], bt.shape[2], _ptr(start), _ptr(lens), int(bool(rope)),
-           float(rope_freq_base), float(rope_freq_scale), _stream())
+    L.call("fmoe_kvcache_append", kc.data_ptr(), vc.data_ptr(), None if ks is None else ks.data_ptr(),
+           None if vs is None else vs.data_ptr(), _TORCH_TO_DT[dtype] if ks is None else L.F8E4M3FN, n_blocks, bs, hkv,
+           d, int(layer), k.data_ptr(), k_stride, v.data_ptr(), v_stride, None if q is None else q.data_ptr(), q_stride,
+           None if out is None else out.data_ptr(), out_stride, n_head, _TORCH_TO_DT[dtype], batch, seq_len,
+           bt.data_ptr(), n_layers, max_blocks, start.data_ptr(), None if lens is None else lens.data_ptr(),
+           int(bool(rope)), float(rope_freq_base), float(rope_freq_scale), _raw_stream(dev))
     if q is None:
         return None
-    if q_out_copy is not None:
-        q_out = q_out_copy.copy_(q_out)
+    if out is not q_out:
+        q_out.copy_(out)
     return _finish(q_out, from_np)
 
 
@@ -189,29 +229,34 @@ def attention_paged(q, k_cache, v_cache, layer: int, block_tables, context_lens,
     up to its own; ``scale`` defaults to ``1 / sqrt(head_dim)``.  Tokens that
     attend nothing, and padding tokens, get zeros.  ``out`` must not overlap
     ``q``."""
-    dev = _device()
+    dev = _here()
     if not isinstance(k_cache, QuantizedKVPool) or not isinstance(v_cache, QuantizedKVPool):
         raise TypeError("attention_paged reads QuantizedKVPool caches")
-    kc, ks, vc, vs = _check_pools(k_cache, v_cache, dev)
-    n_blocks, bs, hkv, d = kc.shape
-    q, q_stride, from_np = _tokens(q, "q", None, d, dev)
-    batch, seq_len, n_head, _ = q.shape
-    bt = _check_tables(block_tables, batch)
-    cl = _ints_to_device(context_lens, "context_lens")
-    if cl.shape != bt.shape[:2]:
-        raise ValueError(f"context_lens must be {tuple(bt.shape[:2])}, got {tuple(cl.shape)}")
-    lens = _per_sequence(seq_lens, "seq_lens", batch)
+    kc, ks, vc, vs, (n_blocks, bs, hkv, d) = _check_pools(k_cache, v_cache, dev)
+    q, q_stride, shape, from_np = _tokens(q, "q", None, d, dev)
+    batch, seq_len, n_head, _ = shape
+    dtype = q.dtype
+    bt, n_layers, max_blocks = _check_tables(block_tables, batch, dev)
+    cl = _ints(context_lens, "context_lens")
+    if cl.shape != (n_layers, batch):
+        raise ValueError(f"context_lens must be [{n_layers}, {batch}], got {tuple(cl.shape)}")
+    if cl.get_device() != dev:
+        raise ValueError(f"context_lens must be on the current device, cuda:{dev}")
+    lens = None if seq_lens is None else _per_sequence(seq_lens, "seq_lens", batch, dev)
     if scale is not None and not float(scale) > 0.0:
         raise ValueError("scale must be positive")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif not isinstance(out, torch.Tensor) or out.dtype != q.dtype or out.shape != q.shape or out.device != dev \
+        out = q.new_empty(shape)
+    elif not isinstance(out, torch.Tensor) or out.dtype is not dtype or out.shape != shape or out.get_device() != dev \
             or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {q.dtype} tensor {tuple(q.shape)} on {dev}")
-    dt, mc = _TORCH_TO_DT[q.dtype], int(max_context_len)
-    nbytes = L.lib().fmoe_attention_paged_workspace_bytes(batch, seq_len, mc, n_head, hkv, d, dt)
-    ws = _workspace(nbytes) if nbytes else None
-    L.call("fmoe_attention_paged", _ptr(q), q_stride, _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs), n_blocks, bs,
-           int(layer), _ptr(bt), _ptr(cl), _ptr(lens), bt.shape[0], batch, seq_len, bt.shape[2], mc, n_head, hkv, d,
-           int(bool(causal)), 0.0 if scale is None else float(scale), dt, _ptr(out), _ptr(ws), nbytes, _stream())
+        raise ValueError(f"out must be a contiguous {dtype} tensor {tuple(shape)} on cuda:{dev}")
+    dt, max_context_len = _TORCH_TO_DT[dtype], int(max_context_len)
+    nbytes = _workspace_bytes(batch, seq_len, max_context_len, n_head, hkv, d, dt)
+    # of this call alone: calls on other streams, and captured ones, share nothing
+    ws = kc.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    L.call("fmoe_attention_paged", q.data_ptr(), q_stride, kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+           n_blocks, bs, int(layer), bt.data_ptr(), cl.data_ptr(), None if lens is None else lens.data_ptr(), n_layers,
+           batch, seq_len, max_blocks, max_context_len, n_head, hkv, d, int(bool(causal)),
+           0.0 if scale is None else float(scale), dt, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+           _raw_stream(dev))
     return _finish(out, from_np)
