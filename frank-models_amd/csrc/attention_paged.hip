@@ -89,20 +89,40 @@ __device__ __forceinline__ int limit_of(const PagedAttnArgs& a, const Span& s, i
 // The n lowest bits.
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0ull; }
 
-__device__ __forceinline__ void store_out(const PagedAttnArgs& a, int64_t i, float v) {
+// Four values from element i on (a multiple of 4) of the output.
+__device__ __forceinline__ void store4(const PagedAttnArgs& a, int64_t i, f32x4_t v) {
   if (a.out_dtype == DT_F32)
-    static_cast<float*>(a.out)[i] = v;
+    *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + i) = v;
   else
-    static_cast<bf16_t*>(a.out)[i] = f32_to_bf16(v);
+    *reinterpret_cast<u32x2_t*>(static_cast<bf16_t*>(a.out) + i) =
+        u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
 }
 
+// Over lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// How a call is cut (plan_of): splits of split_len positions; few rows: the
+// waves that share a row tile.
+struct Plan {
+  bool big;
+  int n_split, split_len, waves_per_tile;
+};
+
 // ------------------------------------------------------------------ few rows
-// Block (row tile of 16, K/V head, context split; sequence): its four waves
-// take chunks of 128 positions in turn, each through a ring of its own in
-// LDS, and are merged at the end.  K and V codes pass through the ring once,
-// by global_load_lds, in tiles that are refilled as soon as they are read, so
-// that loads stay in flight through the arithmetic; so do the page table and
-// the scales of the next chunk.
+// A wave takes one row tile of 16 and, of its context split, every
+// waves_per_tile-th chunk of 64 positions, through a ring of its own in LDS;
+// the waves of a tile are merged at the end.  K and V codes pass through the
+// ring once, by global_load_lds, in tiles that are refilled with the next
+// chunk's as soon as they are read, so that 16 KiB a wave (head_dim 128) stay
+// in flight through the arithmetic, and a wave's first K and V arrive
+// together; the page table runs two chunks ahead, rows and scales one.
 // Scores: v_mfma_f32_16x16x32_bf16 with A = 16 positions x 32 dimensions of
 // K (codes are exact in bf16), B = the 16 query rows: a lane then holds, for
 // row l % 16, positions 4 (l / 16) + i of each 16.  That is the B operand of
@@ -115,21 +135,27 @@ __device__ __forceinline__ void store_out(const PagedAttnArgs& a, int64_t i, flo
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kRows = 16;
-constexpr int kChunk = 128;
+constexpr int kChunk = 64;
 constexpr int kSub = kChunk / 16;  // groups of 16 positions
+
+// The running maximum is raised, and the sums rescaled, only when a row's has
+// grown by more than 2^kLazy: weights are then at most 2^kLazy, which fp32
+// sums and bf16 operands hold as well.
+constexpr float kLazy = 8.f;
 
 template <int D>
 struct Stream {
-  static constexpr int kRowsPerLoad = 1024 / D;                             // a load is 64 lanes x 16 bytes
-  static constexpr int kTile = kRowsPerLoad > 32 ? kRowsPerLoad : 32;       // positions
+  static constexpr int kRowsPerLoad = 1024 / D;                        // a load is 64 lanes x 16 bytes
+  static constexpr int kTile = kRowsPerLoad > 32 ? kRowsPerLoad : 32;  // positions
   static constexpr int kLoads = kTile / kRowsPerLoad;
-  static constexpr int kTiles = kChunk / kTile;
+  static constexpr int kTiles = kChunk / kTile;  // of K, and of V
   static constexpr int kTileB = kTile * D;
-  static constexpr int kRing = kTiles * kTileB;
-  static constexpr int kWaveB = kRing + 4 * kChunk * 4;  // + table, rows, K and V scales of a chunk
-  static constexpr int kChunks16 = D / 16;               // 16-byte pieces of a row
+  static constexpr int kRing = 2 * kTiles * kTileB;
+  static constexpr int kWaveB = kRing + 6 * kChunk * 4;  // + table, rows, and K and V scales of two chunks
+  static constexpr int kPieces = D / 16;                 // 16-byte pieces of a row
   static constexpr int kSteps = D >= 32 ? D / 32 : 1;    // products over the dimensions
   static constexpr int kLds = kWaves * kWaveB + 2 * kWaves * kRows * 4;
+  static_assert(kTiles <= 2, "the waits count at most two tiles");
   static_assert(kRows * D * 4 <= kRing, "a wave's partial output fits its ring");
 };
 
@@ -147,40 +173,58 @@ __device__ __forceinline__ int v_place(int r) {  // rows 0-7 and 16-23, or 8-15 
                    : 0;
 }
 
+// Over lanes l, l ^ 16, l ^ 32 and l ^ 48.
+__device__ __forceinline__ float max_quarters(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_quarters(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 template <int D, int kTerms>
-__global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs a, int n_split, int split_len) {
+__global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs a, Plan plan) {
   using R = Stream<D>;
   constexpr int kL = R::kLoads, kT = R::kTiles;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int q4 = lane >> 4, col = lane & 15;
+  const int wpt = plan.waves_per_tile, part_wave = wave % wpt, tiles = kWaves / wpt;
   const int b = blockIdx.y;
-  const int split = blockIdx.x % n_split, kvh = blockIdx.x / n_split % a.n_head_kv;
-  const int row0 = static_cast<int>(blockIdx.x / n_split / a.n_head_kv) * kRows;
-  const int G = a.n_head / a.n_head_kv;
-  const Span span = span_of(a, b);
-
-  // This lane's query row (column `col` of the products).
-  const int token = (row0 + col) / G, head = kvh * G + (row0 + col) % G;
-  const int limit = limit_of(a, span, token);
-  const int last_token = min((row0 + kRows - 1) / G, span.len - 1);
-  const int first_limit = limit_of(a, span, row0 / G);  // 0: the tile is padding
-  const int end = row0 / G < span.len ? limit_of(a, span, last_token) : 0;
-  const int j0 = split * split_len;
-  const int len = min(split_len, end - j0);  // positions of this block
-  if (len <= 0 && n_split > 1) return;       // the combine reads only the splits with positions
+  const int split = blockIdx.x % plan.n_split, kvh = blockIdx.x / plan.n_split % a.n_head_kv;
+  // the tiles of the last tokens, which attend most, go first
+  const int group = static_cast<int>(gridDim.x / plan.n_split / a.n_head_kv - 1 - blockIdx.x / plan.n_split / a.n_head_kv);
+  const int row0 = (group * tiles + wave / wpt) * kRows;
+  const int j0 = split * plan.split_len;
 
   unsigned char* ring = lds + wave * R::kWaveB;
   int* table = reinterpret_cast<int*>(ring + R::kRing);
   int* rows = table + kChunk;
-  float* ks = reinterpret_cast<float*>(rows + kChunk);
-  float* vs = ks + kChunk;
+  float* ks = reinterpret_cast<float*>(rows + kChunk);  // [2][kChunk]
+  float* vs = ks + 2 * kChunk;                          // [2][kChunk]
   float* stat = reinterpret_cast<float*>(lds + kWaves * R::kWaveB);  // [waves][16] maxima, then sums
 
-  const int n_all = len > 0 ? (len + kChunk - 1) / kChunk : 0;
-  const int n = n_all > wave ? (n_all - wave + kWaves - 1) / kWaves : 0;  // this wave's chunks
+  // Chunk c of this wave: its first position within the sequence.
+  auto chunk_at = [&](int c) __attribute__((always_inline)) { return j0 + (c * wpt + part_wave) * kChunk; };
   const int* seq_table = a.tables + static_cast<int64_t>(b) * a.max_blocks;
+  // The page table entries of a chunk's positions, into LDS.
+  auto load_table = [&](int c) __attribute__((always_inline)) {
+    load_lds4(seq_table + min((chunk_at(c) + lane) / a.block_size, a.max_blocks - 1), table);
+  };
+  load_table(0);  // needs no length, so it is asked for beside them
+
+  // This lane's query row (column `col` of the products).
+  const int G = a.n_head / a.n_head_kv;
+  const Span span = span_of(a, b);
+  const int token = (row0 + col) / G, head = kvh * G + (row0 + col) % G;
+  const int limit = limit_of(a, span, token);
+  const int first_limit = limit_of(a, span, row0 / G);  // 0: the tile is padding
+  const int end = row0 / G < span.len ? limit_of(a, span, min((row0 + kRows - 1) / G, span.len - 1)) : 0;
+  const int len = min(plan.split_len, end - j0);  // positions of this tile in the split
+  const int n_all = len > 0 ? (len + kChunk - 1) / kChunk : 0;
+  const int n = n_all > part_wave ? (n_all - part_wave + wpt - 1) / wpt : 0;  // this wave's chunks
   const int64_t row_b = static_cast<int64_t>(a.n_head_kv) * D;
   const uint8_t* kp = a.k_pool + kvh * D;
   const uint8_t* vp = a.v_pool + kvh * D;
@@ -223,53 +267,31 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
       for (int s = 0; s < R::kSteps; ++s) asm volatile("" : "+v"(q[k][s]));  // loaded here, not between the tiles
   }
 
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f;  // l: of this lane's positions
   f32x4_t acc[D / 16];
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const float c2 = a.scale * kLog2e;
 
-  // Chunk c of this wave: its first position within the sequence.
-  auto chunk_at = [&](int c) { return j0 + (c * kWaves + wave) * kChunk; };
-  // The chunk's page table entries, into LDS (positions past the split's end
-  // read the entry of its last one).
-  auto load_table = [&](int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = min(chunk_at(c) + h * kWave + lane, j0 + len - 1);
-      load_lds4(seq_table + min(j / a.block_size, a.max_blocks - 1), table + h * kWave);
-    }
-  };
-  // Bits of the chunk's positions: a page of the pool, and a row of zeros.
-  uint64_t valid[2], zero[2], valid_now[2], zero_now[2];
+  // Bits of a chunk's positions: a page of the pool, and a row of zeros.
+  uint64_t valid = 0, zero = 0;
   // Pool rows of the chunk, unusable ones replaced by a usable one, and its
   // scales' loads.
   auto load_rows = [&](int c) __attribute__((always_inline)) {
-    int r[2], pb[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = chunk_at(c) + h * kWave + lane;
-      const int lb = t / a.block_size;
-      pb[h] = table[h * kWave + lane];
-      const bool in = t < j0 + len, ok = lb < a.max_blocks && pb[h] >= 0 && pb[h] < a.n_blocks;
-      r[h] = in && ok ? pb[h] * a.block_size + (t - lb * a.block_size) : -1;
-      valid[h] = __ballot(in && ok);
-      zero[h] = __ballot(in && !ok);
-    }
-    const int first = valid[0]   ? __builtin_amdgcn_readlane(r[0], __builtin_ctzll(valid[0]))
-                      : valid[1] ? __builtin_amdgcn_readlane(r[1], __builtin_ctzll(valid[1]))
-                                 : 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool ok = r[h] >= 0;
-      rows[h * kWave + lane] = ok ? r[h] : first;
-      const int64_t at = static_cast<int64_t>(ok ? pb[h] : first / a.block_size) * a.n_head_kv + kvh;
-      load_lds4(a.k_scales + at, ks + h * kWave);
-      load_lds4(a.v_scales + at, vs + h * kWave);
-    }
+    const int t = chunk_at(c) + lane, lb = t / a.block_size;
+    const int pb = table[lane];
+    const bool in = t < j0 + len, ok = in && lb < a.max_blocks && pb >= 0 && pb < a.n_blocks;
+    const int r = ok ? pb * a.block_size + (t - lb * a.block_size) : -1;
+    valid = __ballot(ok);
+    zero = __ballot(in && !ok);
+    const int first = valid ? __builtin_amdgcn_readlane(r, __builtin_ctzll(valid)) : 0;
+    rows[lane] = ok ? r : first;
+    const int64_t at = static_cast<int64_t>(ok ? pb : first / a.block_size) * a.n_head_kv + kvh;
+    load_lds4(a.k_scales + at, ks + (c & 1) * kChunk);
+    load_lds4(a.v_scales + at, vs + (c & 1) * kChunk);
   };
-  const int lr = lane / R::kChunks16, lc = lane % R::kChunks16;  // this lane's row and piece of a load
-  auto load_tile = [&](const uint8_t* pool, int it, bool v) __attribute__((always_inline)) {
+  const int lr = lane / R::kPieces, lc = lane % R::kPieces;  // this lane's row and piece of a load
+  auto load_tile = [&](int it, bool v) __attribute__((always_inline)) {
     int r[kL];
 #pragma unroll
     for (int i = 0; i < kL; ++i) r[i] = rows[it * R::kTile + i * R::kRowsPerLoad + lr];
@@ -277,51 +299,56 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
     for (int i = 0; i < kL; ++i) {
       const int tr = i * R::kRowsPerLoad + lr;
       const int piece = lc ^ (v ? v_place<D>(tr) : k_place<D>(tr));
-      load_lds16(pool + r[i] * row_b + piece * 16, ring + it * R::kTileB + i * 1024);
+      load_lds16((v ? vp : kp) + r[i] * row_b + piece * 16, ring + ((v ? kT : 0) + it) * R::kTileB + i * 1024);
     }
   };
 
   if (n > 0) {
-    load_table(0);
     __builtin_amdgcn_s_waitcnt(wait_vm(0, true));
     asm volatile("" ::: "memory");
     load_rows(0);
+    load_table(1);
     __builtin_amdgcn_s_waitcnt(wait_vm(63, true));
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int it = 0; it < kT; ++it) load_tile(kp, it, false);
+    for (int it = 0; it < kT; ++it) load_tile(it, false);
+#pragma unroll
+    for (int it = 0; it < kT; ++it) load_tile(it, true);
   }
   for (int c = 0; c < n; ++c) {
     const bool more = c + 1 < n;
     const int at = chunk_at(c);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      valid_now[h] = valid[h];
-      zero_now[h] = zero[h];
-    }
-    const bool full = (valid_now[0] & valid_now[1]) == ~0ull && at + kChunk <= first_limit;
+    const bool full = valid == ~0ull && at + kChunk <= first_limit;
     // Positions that this lane's row attends: rows of the pool, and rows of
-    // zeros; bit 16 (st % 4) + i of word st / 4 belongs to score i of sc[st].
-    uint64_t on[2] = {~0ull, ~0ull}, nil[2] = {0ull, 0ull};
+    // zeros; bit 16 st + i belongs to score i of sc[st].
+    uint64_t on = ~0ull, nil = 0ull;
     if (!full) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint64_t below = low_bits(limit - at - 64 * h);
-        on[h] = (valid_now[h] & below) >> (4 * q4);
-        nil[h] = (zero_now[h] & below) >> (4 * q4);
-      }
+      const uint64_t below = low_bits(limit - at);
+      on = (valid & below) >> (4 * q4);
+      nil = (zero & below) >> (4 * q4);
     }
-    auto attends = [&](int st, int i) __attribute__((always_inline)) { return (on[st / 4] >> (16 * (st % 4) + i) & 1) != 0; };
-    load_table(min(c + 1, n - 1));  // always two loads, so that the waits below count alike
+    auto attends = [&](int st, int i) __attribute__((always_inline)) { return (on >> (16 * st + i) & 1) != 0; };
+    const float* ks_now = ks + (c & 1) * kChunk;
+    const float* vs_now = vs + (c & 1) * kChunk;
 
-    // ---- scores.  In flight behind K tile `it`: the tiles after it (K,
-    // then V) and the table
+    // ---- scores.  In flight behind K tile `it`, with another chunk to come:
+    // 2 kT - 1 tiles, and from the first on the next chunk's scales and the
+    // table after it (three loads)
     f32x4_t sc[kSub];
 #pragma unroll
     for (int it = 0; it < kT; ++it) {
-      __builtin_amdgcn_s_waitcnt(wait_vm((kT - 1) * kL + 2, false));
+      if (it == 0)
+        __builtin_amdgcn_s_waitcnt(wait_vm((2 * kT - 1) * kL, false));
+      else if (more)
+        __builtin_amdgcn_s_waitcnt(wait_vm((2 * kT - 1) * kL + 3, false));
+      else
+        __builtin_amdgcn_s_waitcnt(wait_vm((2 * kT - 2) * kL, false));
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("" ::: "memory");
+      if (it == 0 && more) {
+        load_rows(c + 1);  // the table came before this tile
+        load_table(c + 2);
+      }
       constexpr int kSt = R::kTile / 16;
       u32x4_t w[kSt][D >= 64 ? D / 64 : 1];
 #pragma unroll
@@ -334,17 +361,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
             w[u][s] = *reinterpret_cast<const u32x4_t*>(p + (((q4 + 4 * s) ^ k_place<D>(r)) << 4));
         } else {
           const u32x2_t h =
-              *reinterpret_cast<const u32x2_t*>(p + ((((q4 >> 1) ^ k_place<D>(r)) & (R::kChunks16 - 1)) << 4) + 8 * (q4 & 1));
+              *reinterpret_cast<const u32x2_t*>(p + ((((q4 >> 1) ^ k_place<D>(r)) & (R::kPieces - 1)) << 4) + 8 * (q4 & 1));
           w[u][0] = D == 16 && q4 >= 2 ? u32x4_t{0u, 0u, 0u, 0u} : u32x4_t{h[0], h[1], 0u, 0u};
         }
       }
       f32x4_t kscale[kSt];
 #pragma unroll
-      for (int u = 0; u < kSt; ++u) kscale[u] = *reinterpret_cast<const f32x4_t*>(ks + (it * kSt + u) * 16 + 4 * q4);
+      for (int u = 0; u < kSt; ++u) kscale[u] = *reinterpret_cast<const f32x4_t*>(ks_now + (it * kSt + u) * 16 + 4 * q4);
       // the slot is refilled after its reads have returned
       __builtin_amdgcn_s_waitcnt(wait_vm(63, true));
       __builtin_amdgcn_sched_barrier(0);
-      load_tile(vp, it, true);
+      if (more) load_tile(it, false);
 #pragma unroll
       for (int u = 0; u < kSt; ++u) {
         f32x4_t d{0.f, 0.f, 0.f, 0.f};
@@ -359,25 +386,30 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
         for (int i = 0; i < 4; ++i) d[i] *= kscale[u][i];
         if (!full) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            d[i] = attends(st, i) ? d[i] : nil[st / 4] >> (16 * (st % 4) + i) & 1 ? 0.f : -INFINITY;
+          for (int i = 0; i < 4; ++i) d[i] = attends(st, i) ? d[i] : nil >> (16 * st + i) & 1 ? 0.f : -INFINITY;
         }
         sc[st] = d;
       }
     }
 
     // ---- softmax over the wave's positions so far
-    float mx = m;
+    float mx = -INFINITY;
 #pragma unroll
     for (int st = 0; st < kSub; ++st)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[st][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-    const float base = finite_base(mx) * c2;
-    const float f = __builtin_amdgcn_exp2f(fmaf(m, c2, -base));
-    m = mx;
-    float sum = 0.f;
+    mx = max_quarters(mx);
+    if (__any((mx - m) * c2 > kLazy)) {
+      const float top = fmaxf(m, mx);
+      const float f = __builtin_amdgcn_exp2f((m - finite_base(top)) * c2);
+      m = top;
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] *= f;
+    }
+    const float base = finite_base(m) * c2;
     u32x4_t p[kTerms][kSub / 2];
 #pragma unroll
     for (int g = 0; g < kSub / 2; ++g) {
@@ -385,11 +417,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int st = 2 * g + u;
-        const f32x4_t vscale = *reinterpret_cast<const f32x4_t*>(vs + st * 16 + 4 * q4);
+        const f32x4_t vscale = *reinterpret_cast<const f32x4_t*>(vs_now + st * 16 + 4 * q4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float e = __builtin_amdgcn_exp2f(fmaf(sc[st][i], c2, -base));
-          sum += e;
+          l += e;
           w[4 * u + i] = e * vscale[i];
         }
       }
@@ -405,26 +437,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 #pragma unroll
       for (int k = 0; k < kTerms; ++k) p[k][g] = t[k];
     }
-    sum += __shfl_xor(sum, 16, kWave);
-    sum += __shfl_xor(sum, 32, kWave);
-    l = fmaf(l, f, sum);
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] *= f;
 
-    // ---- values.  In flight behind V tile `it`: the V tiles after it and,
-    // with another chunk, its scales and K tiles
+    // ---- values
 #pragma unroll
     for (int it = 0; it < kT; ++it) {
-      if (it == 0)
+      if (more)
+        __builtin_amdgcn_s_waitcnt(wait_vm((2 * kT - 1) * kL + 3, false));
+      else if (it == 0)
         __builtin_amdgcn_s_waitcnt(wait_vm((kT - 1) * kL, false));
-      else if (more)
-        __builtin_amdgcn_s_waitcnt(wait_vm((kT - 1) * kL + 4, false));
-      else if (it == 1)
-        __builtin_amdgcn_s_waitcnt(wait_vm((kT > 2 ? kT - 2 : 0) * kL, false));
-      else if (it == 2)
-        __builtin_amdgcn_s_waitcnt(wait_vm((kT > 3 ? kT - 3 : 0) * kL, false));
       else
         __builtin_amdgcn_s_waitcnt(wait_vm(0, false));
       __builtin_amdgcn_sched_barrier(0);
@@ -434,20 +454,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 #pragma unroll
       for (int g = 0; g < kPg; ++g) {
         const int k = (lane & 15) >> 1, r = 16 * (k >> 2) + 4 * q4 + (k & 3);
-        const unsigned char* tile = ring + it * R::kTileB + (32 * g + r) * D + 8 * (lane & 1);
+        const unsigned char* tile = ring + (kT + it) * R::kTileB + (32 * g + r) * D + 8 * (lane & 1);
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) w[g][t] = read_columns(tile + ((t ^ v_place<D>(r)) << 4));
       }
       __builtin_amdgcn_s_waitcnt(wait_vm(63, true));
       __builtin_amdgcn_sched_barrier(0);
-      if (more) {
-        if (it == 0) {
-          load_rows(c + 1);  // the table came before this tile
-          __builtin_amdgcn_s_waitcnt(wait_vm(63, true));
-          asm volatile("" ::: "memory");
-        }
-        load_tile(kp, it, false);
-      }
+      if (more) load_tile(it, true);
 #pragma unroll
       for (int g = 0; g < kPg; ++g) {
         const int pg = it * kPg + g;
@@ -456,11 +469,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
           uint32_t any = 0;
 #pragma unroll
           for (int t = 0; t < D / 16; ++t) any |= nan_bytes(w[g][t][0]) | nan_bytes(w[g][t][1]);
-          bad = __ballot(any != 0) != 0;
+          bad = __any(any != 0);
         }
         if (__builtin_expect(bad, 0)) {
-          // 1 where this lane's row attends the position
-          float y[8];
+          float y[8];  // 1 where this lane's row attends the position
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = attends(2 * pg + e / 4, e % 4) ? 1.f : 0.f;
           u32x4_t one[1];
@@ -486,42 +498,50 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
       }
     }
   }
-  // nothing of the wave is in flight beyond the table of the last chunk
+  // nothing of the wave is in flight beyond a table
   __builtin_amdgcn_s_waitcnt(wait_vm(0, true));
   asm volatile("" ::: "memory");
 
-  // ---- the waves merged in order
+  // ---- the tile's waves merged in order
   float* o = reinterpret_cast<float*>(ring) + col * D;
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4_t*>(o + 16 * t + 4 * q4) = acc[t];
+  l = sum_quarters(l);
   if (lane < kRows) {
     stat[wave * kRows + lane] = m;
     stat[(kWaves + wave) * kRows + lane] = l;
   }
   __syncthreads();
-  for (int i = tid; i < kRows * D; i += kThreads) {
-    const int r = i / D, d = i % D, t = (row0 + r) / G, h = kvh * G + (row0 + r) % G;
+  if (len <= 0 && plan.n_split > 1) return;  // the join reads only the splits with positions
+  const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
+  for (int i = part_wave * kWave + lane; i < kRows * D / 4; i += wpt * kWave) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4, t = (row0 + r) / G, h = kvh * G + (row0 + r) % G;
     if (t >= a.seq_len) break;
-    float M = stat[r];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, stat[w * kRows + r]);
-    const int64_t zeros = n_split == 1 && t < span.len ? max(a.zero_to - span.cut, 0) : 0;
+    const int w0 = wave - part_wave;
+    float M = stat[w0 * kRows + r];
+    for (int w = 1; w < wpt; ++w) M = fmaxf(M, stat[(w0 + w) * kRows + r]);
+    const int zeros = plan.n_split == 1 && t < span.len ? max(a.zero_to - span.cut, 0) : 0;
     if (zeros > 0) M = fmaxf(M, 0.f);
     const float base = finite_base(M) * c2;
-    float x = 0.f, L = zeros > 0 ? static_cast<float>(zeros) * __builtin_amdgcn_exp2f(-base) : 0.f;
+    f32x4_t x{0.f, 0.f, 0.f, 0.f};
+    float L = zeros > 0 ? static_cast<float>(zeros) * __builtin_amdgcn_exp2f(-base) : 0.f;
+    for (int w = 0; w < wpt; ++w) {
+      const float f = __builtin_amdgcn_exp2f(fmaf(stat[(w0 + w) * kRows + r], c2, -base));  // 0 without positions
+      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(lds + (w0 + w) * R::kWaveB + 16 * i);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(fmaf(stat[w * kRows + r], c2, -base));  // 0 for a wave without positions
-      x = fmaf(f, reinterpret_cast<const float*>(lds + w * R::kWaveB)[i], x);
-      L = fmaf(f, stat[(kWaves + w) * kRows + r], L);
+      for (int e = 0; e < 4; ++e) x[e] = fmaf(f, y[e], x[e]);
+      L = fmaf(f, stat[(kWaves + w0 + w) * kRows + r], L);
     }
     const int64_t row = (static_cast<int64_t>(b) * a.seq_len + t) * a.n_head + h;
-    if (n_split == 1) {
-      store_out(a, row * D + d, t >= span.len || L == 0.f ? 0.f : x / L);
+    if (plan.n_split == 1) {
+      const bool none = t >= span.len || L == 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : x[e] / L;
+      store4(a, row * D + d, x);
     } else {
-      const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
-      a.part[(row * n_split + split) * D + d] = x;
-      if (d < 2) a.part[n_rows * n_split * D + (row * n_split + split) * 2 + d] = d == 0 ? M : L;
+      *reinterpret_cast<f32x4_t*>(a.part + (row * plan.n_split + split) * D + d) = x;
+      if (d == 0)
+        *reinterpret_cast<float2*>(a.part + n_rows * plan.n_split * D + (row * plan.n_split + split) * 2) = float2{M, L};
     }
   }
 }
@@ -540,14 +560,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 // conversion of K.  A lane holds, for row l % 32, positions 8 i + 4 (l / 32)
 // + 0..3, which serve as the B operand of the second product in bf16
 // (32x32x16) with A = V transposed, converted as it is read.
-// The running maximum is raised, and the sums rescaled, only when a row's
-// has grown by more than 2^kLazy: weights are then at most 2^kLazy, which fp32
-// sums and bf16 operands hold as well.
 constexpr int kBigRows = 128;
 constexpr int kWaveRows = 32;
 constexpr int kBigTile = 64;
 constexpr int kStages = 3;
-constexpr float kLazy = 8.f;
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
 
@@ -558,16 +574,6 @@ __device__ __forceinline__ f32x16_t mfma32(const u32x4_t a, const u32x4_t b, f32
 
 __device__ __forceinline__ f32x16_t mfma32_f8(const i32x8_t a, const i32x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
-}
-
-// Maximum of lanes l and l ^ 32.
-__device__ __forceinline__ float max_halves(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_halves(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 template <int D>
@@ -592,9 +598,10 @@ __device__ __forceinline__ int v_place32(int r) {
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a, int n_split, int split_len) {
+__global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a, Plan plan) {
   using R = Big<D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int n_split = plan.n_split, split_len = plan.split_len;
   uint32_t* flags = reinterpret_cast<uint32_t*>(lds + kStages * R::kStageB);  // [stage][wave]: valid, zero << 16
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -912,73 +919,87 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 }
 
 // ------------------------------------------------------------------ joining the splits
-// One wave per output row: the splits that hold positions of it, in order.
-constexpr int kJoinUnroll = 8;
+// D / 4 lanes per output row, four dimensions each, add the splits that hold
+// positions of the row in order.  Bound by latency: the first kJoin splits'
+// statistics and outputs are asked for beside the lengths that say which of
+// them count (the others' memory is there, and not used).
+constexpr int kJoin = 8;
 
 template <int D>
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, int n_split, int split_len) {
-  constexpr int kPer = D > kWave ? D / kWave : 1;  // dimensions of a lane
-  const int lane = threadIdx.x & (kWave - 1);
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, Plan plan) {
+  constexpr int kLanes = D / 4;
   const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
   if (row >= n_rows) return;
+  const int n = plan.n_split, d = threadIdx.x % kLanes * 4;
+  const float* part = a.part + row * n * D + d;
+  const float2* stat = reinterpret_cast<const float2*>(a.part + n_rows * n * D) + row * n;
+  f32x4_t v[kJoin];
+  float2 st[kJoin];
+  auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kJoin; ++u) {
+      const int s = min(s0 + u, n - 1);
+      st[u] = stat[s];
+      v[u] = *reinterpret_cast<const f32x4_t*>(part + static_cast<int64_t>(s) * D);
+    }
+  };
+  load(0);
   const int t = static_cast<int>(row / a.n_head % a.seq_len);
-  const int b = static_cast<int>(row / a.n_head / a.seq_len);
-  const Span span = span_of(a, b);
-  const int used = (limit_of(a, span, t) + split_len - 1) / split_len;
+  const Span span = span_of(a, static_cast<int>(row / a.n_head / a.seq_len));
+  const int used = (limit_of(a, span, t) + plan.split_len - 1) / plan.split_len;
   const int zeros = t < span.len ? max(a.zero_to - span.cut, 0) : 0;
-  const float* part = a.part + row * n_split * D;
-  const float2* stat = reinterpret_cast<const float2*>(a.part + n_rows * n_split * D) + row * n_split;
   const float c2 = a.scale * kLog2e;
-  float M = zeros > 0 ? 0.f : -INFINITY;
-  for (int s = lane; s < used; s += kWave) M = fmaxf(M, stat[s].x);
-  M = wave_max(M);
-  const float base = finite_base(M) * c2;
-  float L = 0.f;
-  for (int s = lane; s < used; s += kWave) L = fmaf(stat[s].y, __builtin_amdgcn_exp2f(fmaf(stat[s].x, c2, -base)), L);
-  L = wave_sum(L) + (zeros > 0 ? static_cast<float>(zeros) * __builtin_amdgcn_exp2f(-base) : 0.f);
-  float o[kPer];
+  float M = zeros > 0 ? 0.f : -INFINITY, L = static_cast<float>(zeros);
+  f32x4_t o{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < used; s0 += kJoin) {
+    if (s0 > 0) load(s0);
+    float top = M;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-  if (lane * kPer < D) {
-    for (int s0 = 0; s0 < used; s0 += kJoinUnroll) {
-      float v[kJoinUnroll][kPer], m[kJoinUnroll];
+    for (int u = 0; u < kJoin; ++u)
+      if (s0 + u < used) top = fmaxf(top, st[u].x);
+    const float base = finite_base(top) * c2, f = __builtin_amdgcn_exp2f(fmaf(M, c2, -base));
+    M = top;
+    L *= f;
 #pragma unroll
-      for (int u = 0; u < kJoinUnroll; ++u) {
-        const int s = min(s0 + u, used - 1);
-        m[u] = stat[s].x;
+    for (int e = 0; e < 4; ++e) o[e] *= f;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) v[u][e] = part[static_cast<int64_t>(s) * D + lane * kPer + e];
-      }
+    for (int u = 0; u < kJoin; ++u) {
+      if (s0 + u < used) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(st[u].x, c2, -base));
+        L = fmaf(st[u].y, w, L);
 #pragma unroll
-      for (int u = 0; u < kJoinUnroll; ++u) {
-        const float f = s0 + u < used ? __builtin_amdgcn_exp2f(fmaf(m[u], c2, -base)) : 0.f;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          if (s0 + u < used) o[e] = fmaf(v[u][e], f, o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(v[u][e], w, o[e]);
       }
     }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) store_out(a, row * D + lane * kPer + e, L == 0.f ? 0.f : o[e] / L);
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = L == 0.f ? 0.f : o[e] / L;
+  store4(a, row * D + d, o);
 }
 
-// Which kernel, and how the context is cut: splits of split_len positions,
-// for two blocks per CU where the rows alone do not give them.
-struct Plan {
-  bool big;
-  int n_split, split_len;
-};
-
+// Which kernel, and how the context is cut: for two blocks per CU where the
+// rows alone do not give them.
 constexpr int kBigFrom = 64;  // query rows of a K/V head
 
 Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int q_dtype) {
   const int64_t rows = static_cast<int64_t>(seq_len) * (n_head / n_head_kv);
+  const int64_t pairs = static_cast<int64_t>(batch) * n_head_kv;
   Plan p;
   p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom;
-  const int tile = p.big ? kBigRows : kRows, step = p.big ? 4 * kBigTile : 2 * kChunk;
-  const int64_t blocks = static_cast<int64_t>(batch) * n_head_kv * ((rows + tile - 1) / tile);
-  int64_t n = blocks > 0 ? (512 + blocks - 1) / blocks : 1;
+  p.waves_per_tile = kWaves;
+  int64_t blocks;
+  int step = 4 * kBigTile;
+  if (p.big) {
+    blocks = pairs * ((rows + kBigRows - 1) / kBigRows);
+  } else {
+    const int64_t tiles = pairs * ((rows + kRows - 1) / kRows);
+    while (p.waves_per_tile > 1 && tiles * p.waves_per_tile > 512 * kWaves) p.waves_per_tile /= 2;
+    blocks = (tiles * p.waves_per_tile + kWaves - 1) / kWaves;
+    step = kChunk * p.waves_per_tile;
+  }
+  int64_t n = blocks > 0 ? 512 / blocks : 1;
+  if (n < 1) n = 1;
   int64_t len = (max_ctx + n - 1) / n;
   len = (len + step - 1) / step * step;
   if (len < step) len = step;
@@ -998,7 +1019,7 @@ void launch_big(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     const int64_t rows = static_cast<int64_t>(a.seq_len) * (a.n_head / a.n_head_kv);
     const int64_t x = (rows + kBigRows - 1) / kBigRows * a.n_head_kv * p.n_split;
     hipLaunchKernelGGL((paged_tile_kernel<D>), dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), lds, s, a,
-                       p.n_split, p.split_len);
+                       p);
   }
 }
 
@@ -1009,9 +1030,10 @@ void launch_stream(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   (void)attr;
   const int64_t rows = static_cast<int64_t>(a.seq_len) * (a.n_head / a.n_head_kv);
-  const int64_t x = (rows + kRows - 1) / kRows * a.n_head_kv * p.n_split;
+  const int64_t group = kRows * (kWaves / p.waves_per_tile);  // rows of a block
+  const int64_t x = (rows + group - 1) / group * a.n_head_kv * p.n_split;
   hipLaunchKernelGGL((paged_stream_kernel<D, kTerms>), dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), lds, s,
-                     a, p.n_split, p.split_len);
+                     a, p);
 }
 
 template <int D>
@@ -1025,8 +1047,8 @@ hipError_t launch_dim(const PagedAttnArgs& a, hipStream_t s) {
     launch_stream<D, 1>(a, p, s);
   if (p.n_split > 1) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
-    hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<unsigned>((rows + kWaves - 1) / kWaves)),
-                       dim3(kThreads), 0, s, a, p.n_split, p.split_len);
+    const int64_t x = (rows * (D / 4) + kThreads - 1) / kThreads;
+    hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<unsigned>(x)), dim3(kThreads), 0, s, a, p);
   }
   return hipGetLastError();
 }
