@@ -8,6 +8,8 @@
 // Query rows of a K/V head are its (token, query head) pairs, token-major:
 // row r is token r / G, query head kvh * G + r % G, for G query heads per
 // K/V head, so that one read of K and V serves the group and the tokens.
+#include <atomic>
+
 #include "common.h"
 #include "launch.h"
 
@@ -108,11 +110,29 @@ __device__ __forceinline__ float sum_halves(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Division of 0 <= x < 2^31 by d: x m / 2^(31 + l) with m = 2^(31 + l) / d
+// rounded up and 2^l >= d, exact because x (m d - 2^(31 + l)) < 2^31 2^l.  The
+// hardware has no integer division; a call's kernels make a dozen before
+// their first load.
+struct Div {
+  uint32_t m, s;
+  static Div by(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return Div{static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d), 31 + l};
+  }
+  __device__ __forceinline__ int operator()(int x) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * m >> s);
+  }
+};
+
 // How a call is cut (plan_of): splits of split_len positions; few rows: the
-// waves that share a row tile.
+// waves that share a row tile, a power of two.
 struct Plan {
   bool big;
   int n_split, split_len, waves_per_tile;
+  int group, tile_groups;  // query heads per K/V head; blocks that its rows take in a split
+  Div split_div, kv_div, group_div, block_div, head_div, len_div;  // n_split, n_head_kv, group, block_size, n_head, split_len
 };
 
 // ------------------------------------------------------------------ few rows
@@ -191,12 +211,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int q4 = lane >> 4, col = lane & 15;
-  const int wpt = plan.waves_per_tile, part_wave = wave % wpt, tiles = kWaves / wpt;
+  const int wpt = plan.waves_per_tile, part_wave = wave & (wpt - 1), tile = wave >> __builtin_ctz(wpt);
   const int b = blockIdx.y;
-  const int split = blockIdx.x % plan.n_split, kvh = blockIdx.x / plan.n_split % a.n_head_kv;
+  const int x = plan.split_div(blockIdx.x), split = blockIdx.x - x * plan.n_split;
+  const int y = plan.kv_div(x), kvh = x - y * a.n_head_kv;
   // the tiles of the last tokens, which attend most, go first
-  const int group = static_cast<int>(gridDim.x / plan.n_split / a.n_head_kv - 1 - blockIdx.x / plan.n_split / a.n_head_kv);
-  const int row0 = (group * tiles + wave / wpt) * kRows;
+  const int row0 = ((plan.tile_groups - 1 - y) * (kWaves >> __builtin_ctz(wpt)) + tile) * kRows;
   const int j0 = split * plan.split_len;
 
   unsigned char* ring = lds + wave * R::kWaveB;
@@ -211,20 +231,21 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   const int* seq_table = a.tables + static_cast<int64_t>(b) * a.max_blocks;
   // The page table entries of a chunk's positions, into LDS.
   auto load_table = [&](int c) __attribute__((always_inline)) {
-    load_lds4(seq_table + min((chunk_at(c) + lane) / a.block_size, a.max_blocks - 1), table);
+    load_lds4(seq_table + min(plan.block_div(chunk_at(c) + lane), a.max_blocks - 1), table);
   };
   load_table(0);  // needs no length, so it is asked for beside them
 
   // This lane's query row (column `col` of the products).
-  const int G = a.n_head / a.n_head_kv;
+  const int G = plan.group;
   const Span span = span_of(a, b);
-  const int token = (row0 + col) / G, head = kvh * G + (row0 + col) % G;
+  const int token = plan.group_div(row0 + col), head = kvh * G + row0 + col - token * G;
   const int limit = limit_of(a, span, token);
-  const int first_limit = limit_of(a, span, row0 / G);  // 0: the tile is padding
-  const int end = row0 / G < span.len ? limit_of(a, span, min((row0 + kRows - 1) / G, span.len - 1)) : 0;
+  const int first_token = plan.group_div(row0);
+  const int first_limit = limit_of(a, span, first_token);  // 0: the tile is padding
+  const int end = first_token < span.len ? limit_of(a, span, min(plan.group_div(row0 + kRows - 1), span.len - 1)) : 0;
   const int len = min(plan.split_len, end - j0);  // positions of this tile in the split
   const int n_all = len > 0 ? (len + kChunk - 1) / kChunk : 0;
-  const int n = n_all > part_wave ? (n_all - part_wave + wpt - 1) / wpt : 0;  // this wave's chunks
+  const int n = n_all > part_wave ? (n_all - part_wave + wpt - 1) >> __builtin_ctz(wpt) : 0;  // this wave's chunks
   const int64_t row_b = static_cast<int64_t>(a.n_head_kv) * D;
   const uint8_t* kp = a.k_pool + kvh * D;
   const uint8_t* vp = a.v_pool + kvh * D;
@@ -278,7 +299,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   // Pool rows of the chunk, unusable ones replaced by a usable one, and its
   // scales' loads.
   auto load_rows = [&](int c) __attribute__((always_inline)) {
-    const int t = chunk_at(c) + lane, lb = t / a.block_size;
+    const int t = chunk_at(c) + lane, lb = plan.block_div(t);
     const int pb = table[lane];
     const bool in = t < j0 + len, ok = in && lb < a.max_blocks && pb >= 0 && pb < a.n_blocks;
     const int r = ok ? pb * a.block_size + (t - lb * a.block_size) : -1;
@@ -286,7 +307,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
     zero = __ballot(in && !ok);
     const int first = valid ? __builtin_amdgcn_readlane(r, __builtin_ctzll(valid)) : 0;
     rows[lane] = ok ? r : first;
-    const int64_t at = static_cast<int64_t>(ok ? pb : first / a.block_size) * a.n_head_kv + kvh;
+    const int64_t at = static_cast<int64_t>(ok ? pb : plan.block_div(first)) * a.n_head_kv + kvh;
     load_lds4(a.k_scales + at, ks + (c & 1) * kChunk);
     load_lds4(a.v_scales + at, vs + (c & 1) * kChunk);
   };
@@ -515,7 +536,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   if (len <= 0 && plan.n_split > 1) return;  // the join reads only the splits with positions
   const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
   for (int i = part_wave * kWave + lane; i < kRows * D / 4; i += wpt * kWave) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4, t = (row0 + r) / G, h = kvh * G + (row0 + r) % G;
+    const int r = i / (D / 4), d = i % (D / 4) * 4, t = plan.group_div(row0 + r), h = kvh * G + row0 + r - t * G;
     if (t >= a.seq_len) break;
     const int w0 = wave - part_wave;
     float M = stat[w0 * kRows + r];
@@ -606,24 +627,24 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int half = lane >> 5, col = lane & 31;
-  const int G = a.n_head / a.n_head_kv;
+  const int G = plan.group;
   const int b = blockIdx.y;
-  const int split = blockIdx.x % n_split, kvh = blockIdx.x / n_split % a.n_head_kv;
+  const int x = plan.split_div(blockIdx.x), split = blockIdx.x - x * n_split;
+  const int y = plan.kv_div(x), kvh = x - y * a.n_head_kv;
   // the tiles of the last tokens, which attend most, go first
-  const int n_tiles = gridDim.x / n_split / a.n_head_kv;
-  const int row0 = (n_tiles - 1 - static_cast<int>(blockIdx.x / n_split / a.n_head_kv)) * kBigRows;
+  const int row0 = (plan.tile_groups - 1 - y) * kBigRows;
   const Span span = span_of(a, b);
 
   const int wave_row0 = row0 + wave * kWaveRows;
-  const int token = (wave_row0 + col) / G, head = kvh * G + (wave_row0 + col) % G;
+  const int token = plan.group_div(wave_row0 + col), head = kvh * G + wave_row0 + col - token * G;
   const int limit = limit_of(a, span, token);
   auto end_of = [&](int first, int n) {  // positions that rows [first, first + n) attend
-    return first / G < span.len ? limit_of(a, span, min((first + n - 1) / G, span.len - 1)) : 0;
+    return plan.group_div(first) < span.len ? limit_of(a, span, min(plan.group_div(first + n - 1), span.len - 1)) : 0;
   };
   const int j0 = split * split_len;
   const int end = min(end_of(row0, kBigRows), j0 + split_len);  // of this block
   const int wave_end = min(end_of(wave_row0, kWaveRows), j0 + split_len);
-  const int first_limit = limit_of(a, span, wave_row0 / G);
+  const int first_limit = limit_of(a, span, plan.group_div(wave_row0));
   const int n = end > j0 ? (end - j0 + kBigTile - 1) / kBigTile : 0;
   if (n == 0 && n_split > 1) return;  // the combine reads only the splits with positions
 
@@ -634,8 +655,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 
   // ---- loads.  Lanes l and l % 16 stand for position 16 wave + l % 16 of a tile.
   const int wp = wave * R::kWaveTileRows + (lane & 15);
-  int next_page = (j0 + wp) / a.block_size, next_off = (j0 + wp) % a.block_size;
-  const int page_step = kBigTile / a.block_size, off_step = kBigTile % a.block_size;
+  int next_page = plan.block_div(j0 + wp), next_off = j0 + wp - next_page * a.block_size;
+  const int page_step = plan.block_div(kBigTile), off_step = kBigTile - page_step * a.block_size;
   int entry = 0;  // table entry of the tile that load_tile takes next
   auto load_entry = [&]() __attribute__((always_inline)) { entry = seq_table[min(next_page, a.max_blocks - 1)]; };
   const int lr = lane / R::kPieces, lc = lane % R::kPieces;
@@ -648,7 +669,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     // unusable rows load a usable one
     const int first = valid ? __builtin_amdgcn_readlane(row, __builtin_ctz(valid)) : 0;
     const int use = row >= 0 ? row : first;
-    const int page = row >= 0 ? entry : first / a.block_size;
+    const int page = row >= 0 ? entry : plan.block_div(first);
     unsigned char* base = lds + stage * R::kStageB;
     if (lane == 0) flags[stage * kWaves + wave] = valid | zero << 16;
     int r[R::kLoads];
@@ -919,58 +940,85 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 }
 
 // ------------------------------------------------------------------ joining the splits
-// D / 4 lanes per output row, four dimensions each, add the splits that hold
-// positions of the row in order.  Bound by latency: the first kJoin splits'
-// statistics and outputs are asked for beside the lengths that say which of
-// them count (the others' memory is there, and not used).
-constexpr int kJoin = 8;
+// D / 4 lanes take four dimensions of an output row each and add the splits
+// that hold positions of it in order; with many splits a whole block takes
+// the row, its groups of lanes every kGroups-th split, and the groups are
+// merged in order.  Bound by latency: the first splits' statistics and
+// outputs are asked for beside the lengths that say which of them count (the
+// others' memory is there, and not used).
+constexpr int kJoin = 8;  // splits of a round
 
-template <int D>
+template <int D, bool kWide>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, Plan plan) {
-  constexpr int kLanes = D / 4;
-  const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
-  if (row >= n_rows) return;
-  const int n = plan.n_split, d = threadIdx.x % kLanes * 4;
+  constexpr int kLanes = D / 4, kGroups = kWide ? kThreads / kLanes : 1;
+  constexpr int kRound = kWide ? 4 : kJoin;
+  __shared__ f32x4_t part_o[kWide ? kThreads : 1];
+  __shared__ float part_m[kGroups], part_l[kGroups];
+  const int n = plan.n_split, d = threadIdx.x % kLanes * 4, g = kWide ? threadIdx.x / kLanes : 0;
+  const int i = kWide ? blockIdx.x : blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;  // (token, head)
+  const int b = blockIdx.y, in_b = a.seq_len * a.n_head;
+  if (i >= in_b) return;  // never with kWide
+  const int64_t row = static_cast<int64_t>(b) * in_b + i;
   const float* part = a.part + row * n * D + d;
-  const float2* stat = reinterpret_cast<const float2*>(a.part + n_rows * n * D) + row * n;
-  f32x4_t v[kJoin];
-  float2 st[kJoin];
+  const float2* stat = reinterpret_cast<const float2*>(a.part + static_cast<int64_t>(a.batch) * in_b * n * D) + row * n;
+  f32x4_t v[kRound];
+  float2 st[kRound];
   auto load = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < kJoin; ++u) {
-      const int s = min(s0 + u, n - 1);
+    for (int u = 0; u < kRound; ++u) {
+      const int s = min(s0 + u * kGroups, n - 1);
       st[u] = stat[s];
       v[u] = *reinterpret_cast<const f32x4_t*>(part + static_cast<int64_t>(s) * D);
     }
   };
-  load(0);
-  const int t = static_cast<int>(row / a.n_head % a.seq_len);
-  const Span span = span_of(a, static_cast<int>(row / a.n_head / a.seq_len));
-  const int used = (limit_of(a, span, t) + plan.split_len - 1) / plan.split_len;
-  const int zeros = t < span.len ? max(a.zero_to - span.cut, 0) : 0;
+  load(g);
+  const int t = plan.head_div(i);
+  const Span span = span_of(a, b);
+  const int limit = limit_of(a, span, t), used = limit > 0 ? plan.len_div(limit - 1) + 1 : 0;
+  const int zeros = t < span.len && g == 0 ? max(a.zero_to - span.cut, 0) : 0;
   const float c2 = a.scale * kLog2e;
   float M = zeros > 0 ? 0.f : -INFINITY, L = static_cast<float>(zeros);
   f32x4_t o{0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < used; s0 += kJoin) {
-    if (s0 > 0) load(s0);
+  for (int s0 = g; s0 < used; s0 += kRound * kGroups) {
+    if (s0 > g) load(s0);
     float top = M;
 #pragma unroll
-    for (int u = 0; u < kJoin; ++u)
-      if (s0 + u < used) top = fmaxf(top, st[u].x);
+    for (int u = 0; u < kRound; ++u)
+      if (s0 + u * kGroups < used) top = fmaxf(top, st[u].x);
     const float base = finite_base(top) * c2, f = __builtin_amdgcn_exp2f(fmaf(M, c2, -base));
     M = top;
     L *= f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= f;
 #pragma unroll
-    for (int u = 0; u < kJoin; ++u) {
-      if (s0 + u < used) {
+    for (int u = 0; u < kRound; ++u) {
+      if (s0 + u * kGroups < used) {
         const float w = __builtin_amdgcn_exp2f(fmaf(st[u].x, c2, -base));
         L = fmaf(st[u].y, w, L);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(v[u][e], w, o[e]);
       }
+    }
+  }
+  if constexpr (kWide) {
+    part_o[threadIdx.x] = o;
+    if (d == 0) {
+      part_m[g] = M;
+      part_l[g] = L;
+    }
+    __syncthreads();
+    if (g > 0) return;
+#pragma unroll 4
+    for (int k = 1; k < kGroups; ++k) M = fmaxf(M, part_m[k]);
+    const float base = finite_base(M) * c2;
+    L = 0.f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < kGroups; ++k) {
+      const float w = __builtin_amdgcn_exp2f(fmaf(part_m[k], c2, -base));
+      L = fmaf(part_l[k], w, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(part_o[k * kLanes + threadIdx.x][e], w, o[e]);
     }
   }
 #pragma unroll
@@ -982,7 +1030,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, P
 // rows alone do not give them.
 constexpr int kBigFrom = 64;  // query rows of a K/V head
 
-Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int q_dtype) {
+Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int block_size, int q_dtype) {
   const int64_t rows = static_cast<int64_t>(seq_len) * (n_head / n_head_kv);
   const int64_t pairs = static_cast<int64_t>(batch) * n_head_kv;
   Plan p;
@@ -1006,49 +1054,55 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
   n = (max_ctx + len - 1) / len;
   p.n_split = static_cast<int>(n < 1 ? 1 : n);
   p.split_len = static_cast<int>(len);
+  p.group = n_head / n_head_kv;
+  const int64_t block_rows = p.big ? kBigRows : kRows * (kWaves / p.waves_per_tile);
+  p.tile_groups = static_cast<int>((rows + block_rows - 1) / block_rows);
+  p.split_div = Div::by(p.n_split);
+  p.kv_div = Div::by(n_head_kv);
+  p.group_div = Div::by(p.group);
+  p.block_div = Div::by(block_size);
+  p.head_div = Div::by(n_head);
+  p.len_div = Div::by(p.split_len);
   return p;
 }
 
-template <int D>
-void launch_big(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
-  if constexpr (D >= 64) {
-    constexpr int lds = Big<D>::kLds;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_tile_kernel<D>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    (void)attr;
-    const int64_t rows = static_cast<int64_t>(a.seq_len) * (a.n_head / a.n_head_kv);
-    const int64_t x = (rows + kBigRows - 1) / kBigRows * a.n_head_kv * p.n_split;
-    hipLaunchKernelGGL((paged_tile_kernel<D>), dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), lds, s, a,
-                       p);
+// More LDS than 64 KiB is asked for once per kernel and device.
+template <auto kKernel, int kLds>
+hipError_t launch_attn(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
+  static std::atomic<uint64_t> asked{0};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(asked.load(std::memory_order_relaxed) & bit)) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess) return e;
+    asked.fetch_or(bit, std::memory_order_relaxed);
   }
-}
-
-template <int D, int kTerms>
-void launch_stream(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
-  constexpr int lds = Stream<D>::kLds;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_stream_kernel<D, kTerms>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  (void)attr;
-  const int64_t rows = static_cast<int64_t>(a.seq_len) * (a.n_head / a.n_head_kv);
-  const int64_t group = kRows * (kWaves / p.waves_per_tile);  // rows of a block
-  const int64_t x = (rows + group - 1) / group * a.n_head_kv * p.n_split;
-  hipLaunchKernelGGL((paged_stream_kernel<D, kTerms>), dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), lds, s,
-                     a, p);
+  const int64_t x = static_cast<int64_t>(p.tile_groups) * a.n_head_kv * p.n_split;
+  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), kLds, s, a, p);
+  return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_dim(const PagedAttnArgs& a, hipStream_t s) {
-  const Plan p = plan_of(a.batch, a.seq_len, a.max_ctx, a.n_head, a.n_head_kv, D, a.q_dtype);
-  if (p.big)
-    launch_big<D>(a, p, s);
-  else if (a.q_dtype == DT_F32)
-    launch_stream<D, 3>(a, p, s);
-  else
-    launch_stream<D, 1>(a, p, s);
+  const Plan p = plan_of(a.batch, a.seq_len, a.max_ctx, a.n_head, a.n_head_kv, D, a.block_size, a.q_dtype);
+  hipError_t e = hipErrorNotSupported;
+  if (p.big) {
+    if constexpr (D >= 64) e = launch_attn<paged_tile_kernel<D>, Big<D>::kLds>(a, p, s);
+  } else if (a.q_dtype == DT_F32) {
+    e = launch_attn<paged_stream_kernel<D, 3>, Stream<D>::kLds>(a, p, s);
+  } else {
+    e = launch_attn<paged_stream_kernel<D, 1>, Stream<D>::kLds>(a, p, s);
+  }
+  if (e != hipSuccess) return e;
   if (p.n_split > 1) {
-    const int64_t rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
-    const int64_t x = (rows * (D / 4) + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL((paged_join_kernel<D>), dim3(static_cast<unsigned>(x)), dim3(kThreads), 0, s, a, p);
+    const int rows = a.seq_len * a.n_head, per_block = kThreads / (D / 4);
+    if (p.n_split > kJoin)
+      hipLaunchKernelGGL((paged_join_kernel<D, true>), dim3(rows, a.batch), dim3(kThreads), 0, s, a, p);
+    else
+      hipLaunchKernelGGL((paged_join_kernel<D, false>), dim3((rows + per_block - 1) / per_block, a.batch),
+                         dim3(kThreads), 0, s, a, p);
   }
   return hipGetLastError();
 }
@@ -1061,7 +1115,7 @@ bool paged_attn_supported(int head_dim) {
 
 size_t paged_attn_workspace_floats(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim,
                                    int q_dtype) {
-  const Plan p = plan_of(batch, seq_len, max_ctx, n_head, n_head_kv, head_dim, q_dtype);
+  const Plan p = plan_of(batch, seq_len, max_ctx, n_head, n_head_kv, head_dim, 1, q_dtype);
   if (p.n_split <= 1) return 0;
   return static_cast<size_t>(batch) * seq_len * n_head * p.n_split * (head_dim + 2);
 }
