@@ -131,7 +131,7 @@ struct Div {
 struct Plan {
   bool big;
   int n_split, split_len, waves_per_tile;
-  int group, tile_groups;  // query heads per K/V head; blocks that its rows take in a split
+  int group, tile_groups;  // query heads per K/V head; blocks that a sequence's rows take in a split
   Div split_div, kv_div, group_div, block_div, head_div, len_div;  // n_split, n_head_kv, group, block_size, n_head, split_len
 };
 
@@ -211,12 +211,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int q4 = lane >> 4, col = lane & 15;
-  const int wpt = plan.waves_per_tile, part_wave = wave & (wpt - 1), tile = wave >> __builtin_ctz(wpt);
+  const int wpt = plan.waves_per_tile, part_wave = wave & (wpt - 1), tiles_log2 = __builtin_ctz(kWaves / wpt);
   const int b = blockIdx.y;
-  const int x = plan.split_div(blockIdx.x), split = blockIdx.x - x * plan.n_split;
-  const int y = plan.kv_div(x), kvh = x - y * a.n_head_kv;
-  // the tiles of the last tokens, which attend most, go first
-  const int row0 = ((plan.tile_groups - 1 - y) * (kWaves >> __builtin_ctz(wpt)) + tile) * kRows;
+  const int g = plan.split_div(blockIdx.x), split = blockIdx.x - g * plan.n_split;
+  // Row tiles by (rows, K/V head), heads fastest: a block's waves read
+  // neighbouring heads' parts of the same pool rows, 512 bytes together.  The
+  // tiles of the last tokens, which attend most, go first.
+  const int tile = ((plan.tile_groups - 1 - g) << tiles_log2) + (wave >> (2 - tiles_log2));
+  const int row_tile = plan.kv_div(tile), kvh = tile - row_tile * a.n_head_kv;
+  const int row0 = row_tile * kRows;
   const int j0 = split * plan.split_len;
 
   unsigned char* ring = lds + wave * R::kWaveB;
@@ -632,7 +635,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   const int x = plan.split_div(blockIdx.x), split = blockIdx.x - x * n_split;
   const int y = plan.kv_div(x), kvh = x - y * a.n_head_kv;
   // the tiles of the last tokens, which attend most, go first
-  const int row0 = (plan.tile_groups - 1 - y) * kBigRows;
+  const int row0 = (plan.kv_div(plan.tile_groups) - 1 - y) * kBigRows;
   const Span span = span_of(a, b);
 
   const int wave_row0 = row0 + wave * kWaveRows;
@@ -1035,18 +1038,31 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
   const int64_t pairs = static_cast<int64_t>(batch) * n_head_kv;
   Plan p;
   p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom;
-  p.waves_per_tile = kWaves;
-  int64_t blocks;
-  int step = 4 * kBigTile;
+  int64_t blocks, n;
+  int step;
   if (p.big) {
+    p.waves_per_tile = 1;
     blocks = pairs * ((rows + kBigRows - 1) / kBigRows);
+    n = 512 / blocks;
+    step = 4 * kBigTile;
   } else {
-    const int64_t tiles = pairs * ((rows + kRows - 1) / kRows);
-    while (p.waves_per_tile > 1 && tiles * p.waves_per_tile > 512 * kWaves) p.waves_per_tile /= 2;
-    blocks = (tiles * p.waves_per_tile + kWaves - 1) / kWaves;
+    // About 1024 waves, one per SIMD, which keep the memory as busy as twice
+    // as many (64 x 8192 positions 176 against 171 us) and spend half the
+    // prologues.  Two waves of a tile and two heads per block rather than
+    // four and one (64 x 8192: 201 us, 16 x 4096: 30.6 against 33.2 us; half
+    // of the pool rows' neighbouring parts are read together), until there
+    // are so many splits that joining them costs more (1 x 32768: 27 against
+    // 21 us); one where the tiles alone are enough.
+    const int64_t tiles = n_head_kv * ((rows + kRows - 1) / kRows);
+    p.waves_per_tile = batch * tiles >= 2048 ? 1 : 2;
+    n = 512 / (batch * tiles);
+    if (n > 16) {
+      p.waves_per_tile = 4;
+      n /= 2;
+    }
+    blocks = batch * ((tiles * p.waves_per_tile + kWaves - 1) / kWaves);
     step = kChunk * p.waves_per_tile;
   }
-  int64_t n = blocks > 0 ? 512 / blocks : 1;
   if (n < 1) n = 1;
   int64_t len = (max_ctx + n - 1) / n;
   len = (len + step - 1) / step * step;
@@ -1055,8 +1071,7 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
   p.n_split = static_cast<int>(n < 1 ? 1 : n);
   p.split_len = static_cast<int>(len);
   p.group = n_head / n_head_kv;
-  const int64_t block_rows = p.big ? kBigRows : kRows * (kWaves / p.waves_per_tile);
-  p.tile_groups = static_cast<int>((rows + block_rows - 1) / block_rows);
+  p.tile_groups = static_cast<int>(blocks / batch);
   p.split_div = Div::by(p.n_split);
   p.kv_div = Div::by(n_head_kv);
   p.group_div = Div::by(p.group);
@@ -1079,7 +1094,7 @@ hipError_t launch_attn(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     if (e != hipSuccess) return e;
     asked.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int64_t x = static_cast<int64_t>(p.tile_groups) * a.n_head_kv * p.n_split;
+  const int64_t x = static_cast<int64_t>(p.tile_groups) * p.n_split;
   hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), kLds, s, a, p);
   return hipGetLastError();
 }
@@ -1115,6 +1130,7 @@ bool paged_attn_supported(int head_dim) {
 
 size_t paged_attn_workspace_floats(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim,
                                    int q_dtype) {
+  if (batch == 0 || seq_len == 0) return 0;
   const Plan p = plan_of(batch, seq_len, max_ctx, n_head, n_head_kv, head_dim, 1, q_dtype);
   if (p.n_split <= 1) return 0;
   return static_cast<size_t>(batch) * seq_len * n_head * p.n_split * (head_dim + 2);
