@@ -129,10 +129,10 @@ struct Div {
 // How a call is cut (plan_of): splits of split_len positions; few rows: the
 // waves that share a row tile, a power of two.
 struct Plan {
-  bool big;
+  bool big, aligned;  // aligned: four neighbouring positions share a page
   int n_split, split_len, waves_per_tile;
   int group, tile_groups;  // query heads per K/V head; blocks that a sequence's rows take in a split
-  Div split_div, kv_div, group_div, block_div, head_div, len_div;  // n_split, n_head_kv, group, block_size, n_head, split_len
+  Div batch_div, split_div, kv_div, group_div, block_div, head_div, len_div;  // batch, n_split, n_head_kv, group, block_size, n_head, split_len
 };
 
 // ------------------------------------------------------------------ few rows
@@ -212,8 +212,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int q4 = lane >> 4, col = lane & 15;
   const int wpt = plan.waves_per_tile, part_wave = wave & (wpt - 1), tiles_log2 = __builtin_ctz(kWaves / wpt);
-  const int b = blockIdx.y;
-  const int g = plan.split_div(blockIdx.x), split = blockIdx.x - g * plan.n_split;
+  const int x = plan.split_div(blockIdx.x), split = blockIdx.x - x * plan.n_split;
+  const int g = plan.batch_div(x), b = x - g * a.batch;
   // Row tiles by (rows, K/V head), heads fastest: a block's waves read
   // neighbouring heads' parts of the same pool rows, 512 bytes together.  The
   // tiles of the last tokens, which attend most, go first.
@@ -596,8 +596,29 @@ __device__ __forceinline__ f32x16_t mfma32(const u32x4_t a, const u32x4_t b, f32
                                                 0, 0, 0);
 }
 
-__device__ __forceinline__ f32x16_t mfma32_f8(const i32x8_t a, const i32x8_t b, f32x16_t c) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+// a times 2^(scale - 127), one scale for each lane's part of a row.
+__device__ __forceinline__ f32x16_t mfma32_f8(const i32x8_t a, int scale, const i32x8_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, scale, 0, 127);
+}
+
+__device__ __forceinline__ bool is_pow2(float v) {  // positive, normal
+  const uint32_t u = __float_as_uint(v);
+  return (u & 0x7FFFFFu) == 0 && u - 0x800000u < 0x7F000000u;
+}
+
+// Four codes times s (a power of two), then four times t, in bf16.
+__device__ __forceinline__ u32x4_t scaled_bf16x8(uint32_t a, float s, uint32_t b, float t) {
+  return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, t, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, t, true))};
+}
+
+// s plus both halves of w.
+__device__ __forceinline__ float add_bf16x2(uint32_t w, float s) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+  const bf16x2_t one = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), one, s, false);
 }
 
 template <int D>
@@ -631,11 +652,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int half = lane >> 5, col = lane & 31;
   const int G = plan.group;
-  const int b = blockIdx.y;
   const int x = plan.split_div(blockIdx.x), split = blockIdx.x - x * n_split;
-  const int y = plan.kv_div(x), kvh = x - y * a.n_head_kv;
-  // the tiles of the last tokens, which attend most, go first
-  const int row0 = (plan.kv_div(plan.tile_groups) - 1 - y) * kBigRows;
+  const int g = plan.batch_div(x), b = x - g * a.batch;
+  // the tiles of the last tokens, which attend most, go first, in every sequence
+  const int tile = plan.tile_groups - 1 - g, row_tile = plan.kv_div(tile), kvh = tile - row_tile * a.n_head_kv;
+  const int row0 = row_tile * kBigRows;
   const Span span = span_of(a, b);
 
   const int wave_row0 = row0 + wave * kWaveRows;
@@ -785,6 +806,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
       nil[1] = static_cast<uint32_t>(z >> 32);
     }
 
+    // Scales that are powers of two, one for four neighbouring positions, cost
+    // nothing: the products take K's, the conversion of V takes V's.  Others
+    // multiply scores and weights.
+    const float* k_of = scales + (col >> 4) * kWave + (col & 15);  // of position col of each 32
+    const float ks[2] = {k_of[0], k_of[2 * kWave]};
+    const bool pow2 =
+        plan.aligned && !__any(!is_pow2(ks[0]) || !is_pow2(ks[1]) || !is_pow2(scales[(lane >> 4) * kWave + 16 + (lane & 15)]));
+    float vs[8];  // of positions 8 g + 4 half + 0..3
+#pragma unroll
+    for (int g = 0; g < 8; ++g) vs[g] = pow2 ? scales[(g >> 1) * kWave + 16 + 8 * (g & 1) + 4 * half] : 1.f;
+
     // ---- scores
     f32x16_t sc[2];
 #pragma unroll
@@ -792,6 +824,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[pt][i] = 0.f;
       const int r = 32 * pt + col;
+      const int e8m0 = pow2 ? static_cast<int>(__float_as_uint(ks[pt]) >> 23) : 127;
 #pragma unroll
       for (int s = 0; s < D / 64; ++s) {
         u32x4_t w[2];
@@ -799,19 +832,16 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
         for (int e = 0; e < 2; ++e)
           w[e] = *reinterpret_cast<const u32x4_t*>(base + r * D + (((4 * s + 2 * half + e) ^ k_place<D>(r)) << 4));
         const i32x8_t k = __builtin_bit_cast(i32x8_t, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        sc[pt] = mfma32_f8(k, qh[s], sc[pt]);
-        sc[pt] = mfma32_f8(k, ql[s], sc[pt]);
+        sc[pt] = mfma32_f8(k, e8m0, qh[s], sc[pt]);
+        sc[pt] = mfma32_f8(k, e8m0, ql[s], sc[pt]);
       }
     }
-    float mx = -INFINITY;
+    if (!pow2) {
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt)
+      for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4_t ks = *reinterpret_cast<const f32x4_t*>(scales + (2 * pt + g / 2) * kWave + 8 * (g % 2) + 4 * half);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[pt][4 * g + i] *= ks[i];
-      }
+        for (int i = 0; i < 16; ++i) sc[pt][i] *= scales[(2 * pt + (i >> 3)) * kWave + 8 * (i >> 2 & 1) + 4 * half + (i & 3)];
+    }
     if (!full) {
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt)
@@ -821,6 +851,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
           sc[pt][i] = on[pt] & bit ? sc[pt][i] : nil[pt] & bit ? 0.f : -INFINITY;
         }
     }
+    float mx = -INFINITY;
 #pragma unroll
     for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
@@ -845,25 +876,39 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     for (int pt = 0; pt < 2; ++pt) {
       float w[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4_t vs =
-            *reinterpret_cast<const f32x4_t*>(scales + (2 * pt + g / 2) * kWave + 16 + 8 * (g % 2) + 4 * half);
+      for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(sc[pt][i], c2, -mc));
+      if (!pow2) {
+        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(sc[pt][4 * g + i], c2, -mc));
-          l += e;
-          w[4 * g + i] = e * vs[i];
+        for (int i = 0; i < 16; ++i) {
+          sum += w[i];
+          w[i] *= scales[(2 * pt + (i >> 3)) * kWave + 16 + 8 * (i >> 2 & 1) + 4 * half + (i & 3)];
         }
+        l += sum;
       }
-      if (!full) {
+      if (!full && !pow2) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (!(on[pt] & 1u << (8 * (i >> 2) + (i & 3)))) w[i] = 0.f;  // 0 times a scale that is not finite
       }
       split8<1>(w, &p[2 * pt]);
       split8<1>(w + 8, &p[2 * pt + 1]);
+      if (pow2) {  // the sum of the weights as they are multiplied, rounded to bf16
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) l = add_bf16x2(p[2 * pt + g][e], l);
+        if (!full) {  // a row of zeros has its weight and no value
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t bits = on[pt] >> (8 * (2 * g + (e >> 1)) + 2 * (e & 1));
+              p[2 * pt + g][e] &= (bits & 1 ? 0xFFFFu : 0u) | (bits & 2 ? 0xFFFF0000u : 0u);
+            }
+        }
+      }
     }
-
     __builtin_amdgcn_sched_barrier(0);
 
     // ---- values
@@ -901,7 +946,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
         }
       }
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) acc[d] = mfma32(f8x8_to_bf16x8(w[d][0], w[d][1]), p[s], acc[d]);
+      for (int d = 0; d < D / 32; ++d)
+        acc[d] = mfma32(scaled_bf16x8(w[d][0], vs[2 * s], w[d][1], vs[2 * s + 1]), p[s], acc[d]);
     }
   }
   __builtin_amdgcn_s_waitcnt(wait_vm(0, true));  // the loads past the end
@@ -1037,6 +1083,7 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
   const int64_t rows = static_cast<int64_t>(seq_len) * (n_head / n_head_kv);
   const int64_t pairs = static_cast<int64_t>(batch) * n_head_kv;
   Plan p;
+  p.aligned = block_size % 4 == 0;
   p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom;
   int64_t blocks, n;
   int step;
@@ -1072,6 +1119,7 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
   p.split_len = static_cast<int>(len);
   p.group = n_head / n_head_kv;
   p.tile_groups = static_cast<int>(blocks / batch);
+  p.batch_div = Div::by(batch);
   p.split_div = Div::by(p.n_split);
   p.kv_div = Div::by(n_head_kv);
   p.group_div = Div::by(p.group);
@@ -1094,8 +1142,9 @@ hipError_t launch_attn(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     if (e != hipSuccess) return e;
     asked.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int64_t x = static_cast<int64_t>(p.tile_groups) * p.n_split;
-  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(x), a.batch), dim3(kThreads), kLds, s, a, p);
+  const int64_t x = static_cast<int64_t>(p.tile_groups) * a.batch * p.n_split;
+  if (x > INT32_MAX) return hipErrorInvalidValue;  // the entry points bound it
+  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(x)), dim3(kThreads), kLds, s, a, p);
   return hipGetLastError();
 }
 

@@ -1698,6 +1698,7 @@ int fmoe_attention_paged(const void* q, int64_t q_stride, const void* k_cache, c
   if (n_head % n_head_kv) return fail(FMOE_ERR_SHAPE, "n_head %% n_head_kv != 0");
   FMOE_TRY(check_dims("max_context_len", max_context_len, 0, kMaxPagedContext));
   if (seq_len > 0) FMOE_TRY(check_dims("seq_len", seq_len, 0, kMaxPagedContext / n_head));
+  if (batch * seq_len * n_head > (1ll << 34)) return fail(FMOE_ERR_SHAPE, "batch * seq_len * n_head exceeds 2^34");
   if (causal != 0 && causal != 1) return fail(FMOE_ERR_INVALID_ARGUMENT, "causal must be 0 or 1");
   if (!(scale >= 0.f && std::isfinite(scale)))
     return fail(FMOE_ERR_INVALID_ARGUMENT, "scale must be positive and finite (0: 1/sqrt(head_dim))");
