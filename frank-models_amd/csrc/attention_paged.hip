@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   const int len = min(plan.split_len, end - j0);  // positions of this tile in the split
   const int n_all = len > 0 ? (len + kChunk - 1) / kChunk : 0;
   const int n = n_all > part_wave ? (n_all - part_wave + wpt - 1) >> __builtin_ctz(wpt) : 0;  // this wave's chunks
-  const int64_t row_b = static_cast<int64_t>(a.n_head_kv) * D;
+  const uint32_t row_b = static_cast<uint32_t>(a.n_head_kv) * D;
   const uint8_t* kp = a.k_pool + kvh * D;
   const uint8_t* vp = a.v_pool + kvh * D;
 
@@ -316,14 +316,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
   };
   const int lr = lane / R::kPieces, lc = lane % R::kPieces;  // this lane's row and piece of a load
   auto load_tile = [&](int it, bool v) __attribute__((always_inline)) {
-    int r[kL];
+    uint32_t r[kL];
 #pragma unroll
     for (int i = 0; i < kL; ++i) r[i] = rows[it * R::kTile + i * R::kRowsPerLoad + lr];
 #pragma unroll
     for (int i = 0; i < kL; ++i) {
       const int tr = i * R::kRowsPerLoad + lr;
       const int piece = lc ^ (v ? v_place<D>(tr) : k_place<D>(tr));
-      load_lds16((v ? vp : kp) + r[i] * row_b + piece * 16, ring + ((v ? kT : 0) + it) * R::kTileB + i * 1024);
+      load_lds16((v ? vp : kp) + piece * 16 + static_cast<uint64_t>(r[i]) * row_b, ring + ((v ? kT : 0) + it) * R::kTileB + i * 1024);
     }
   };
 
@@ -601,11 +601,6 @@ __device__ __forceinline__ f32x16_t mfma32_f8(const i32x8_t a, int scale, const 
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, scale, 0, 127);
 }
 
-__device__ __forceinline__ bool is_pow2(float v) {  // positive, normal
-  const uint32_t u = __float_as_uint(v);
-  return (u & 0x7FFFFFu) == 0 && u - 0x800000u < 0x7F000000u;
-}
-
 // Four codes times s (a power of two), then four times t, in bf16.
 __device__ __forceinline__ u32x4_t scaled_bf16x8(uint32_t a, float s, uint32_t b, float t) {
   return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false)),
@@ -629,8 +624,8 @@ struct Big {
   static constexpr int kTileB = kBigTile * D;
   static constexpr int kScaleB = kWaves * kWave * 4;
   static constexpr int kStageB = 2 * kTileB + kScaleB;
-  static constexpr int kLds = kStages * kStageB + kStages * kWaves * 4;
-  static constexpr int kPerTile = 2 * kLoads + 1;  // loads per wave and tile
+  static constexpr int kLds = kStages * kStageB + kThreads * 4 + kStages * kWaves * 4;
+  static constexpr int kPerTile = 2 * kLoads + 2;  // loads per wave and tile, the entries of the next first
   static constexpr int kWaveTileRows = kBigTile / kWaves;
   static_assert(kLoads * kRowsPerLoad == kWaveTileRows, "a wave loads whole rows");
 };
@@ -647,7 +642,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   using R = Big<D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int n_split = plan.n_split, split_len = plan.split_len;
-  uint32_t* flags = reinterpret_cast<uint32_t*>(lds + kStages * R::kStageB);  // [stage][wave]: valid, zero << 16
+  uint32_t* flags = reinterpret_cast<uint32_t*>(lds + kStages * R::kStageB + kThreads * 4);  // [stage][wave]: valid, zero << 16
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int half = lane >> 5, col = lane & 31;
@@ -673,48 +668,62 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   if (n == 0 && n_split > 1) return;  // the combine reads only the splits with positions
 
   const int* seq_table = a.tables + static_cast<int64_t>(b) * a.max_blocks;
-  const int64_t row_b = static_cast<int64_t>(a.n_head_kv) * D;
+  const uint32_t row_b = static_cast<uint32_t>(a.n_head_kv) * D;
   const uint8_t* kp = a.k_pool + kvh * D;
   const uint8_t* vp = a.v_pool + kvh * D;
 
-  // ---- loads.  Lanes l and l % 16 stand for position 16 wave + l % 16 of a tile.
+  // ---- loads.  Lanes l and l % 16 stand for position 16 wave + l % 16 of a
+  // tile.  All of them go to LDS, the table entries of a tile too, ahead of
+  // the loads of the tile before it: the compiler, which would wait for a
+  // register, leaves the counting to the waits below.
   const int wp = wave * R::kWaveTileRows + (lane & 15);
-  int next_page = plan.block_div(j0 + wp), next_off = j0 + wp - next_page * a.block_size;
+  int next_j = j0 + wp, next_page = plan.block_div(next_j), next_off = next_j - next_page * a.block_size;
   const int page_step = plan.block_div(kBigTile), off_step = kBigTile - page_step * a.block_size;
-  int entry = 0;  // table entry of the tile that load_tile takes next
-  auto load_entry = [&]() __attribute__((always_inline)) { entry = seq_table[min(next_page, a.max_blocks - 1)]; };
+  int* entries = reinterpret_cast<int*>(lds + kStages * R::kStageB) + wave * kWave;
+  auto load_entries = [&]() __attribute__((always_inline)) {
+    load_lds4(seq_table + min(next_page, a.max_blocks - 1), entries);
+  };
   const int lr = lane / R::kPieces, lc = lane % R::kPieces;
-  int next_j = j0 + wp;
+  const float* scales_of = (lane & 16 ? a.v_scales : a.k_scales) + kvh;
+  const uint8_t *k_at[R::kLoads], *v_at[R::kLoads];
+#pragma unroll
+  for (int i = 0; i < R::kLoads; ++i) {
+    const int tr = wave * R::kWaveTileRows + i * R::kRowsPerLoad + lr;
+    k_at[i] = kp + ((lc ^ k_place<D>(tr)) << 4);
+    v_at[i] = vp + ((lc ^ v_place32<D>(tr)) << 4);
+  }
   auto load_tile = [&](int stage) __attribute__((always_inline)) {
-    const bool in = next_j < end, ok = next_page < a.max_blocks && entry >= 0 && entry < a.n_blocks;
-    const int row = in && ok ? entry * a.block_size + next_off : -1;
-    const uint32_t valid = static_cast<uint32_t>(__ballot(row >= 0)) & 0xFFFFu;
-    const uint32_t zero = static_cast<uint32_t>(__ballot(in && !ok)) & 0xFFFFu;
-    // unusable rows load a usable one
-    const int first = valid ? __builtin_amdgcn_readlane(row, __builtin_ctz(valid)) : 0;
-    const int use = row >= 0 ? row : first;
-    const int page = row >= 0 ? entry : plan.block_div(first);
+    const int entry = entries[lane];
+    const bool in = next_j < end;
+    const bool ok = (next_page < a.max_blocks) & (static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.n_blocks)) & in;
+    const uint32_t valid = static_cast<uint32_t>(__ballot(ok)) & 0xFFFFu;
+    const uint32_t zero = static_cast<uint32_t>(__ballot(in & !ok)) & 0xFFFFu;
+    // unusable rows load a usable one (page 0 is there)
+    const int from = valid ? __builtin_ctz(valid) : 0;
+    const int some_page = valid ? __builtin_amdgcn_readlane(entry, from) : 0;
+    const int some_off = valid ? __builtin_amdgcn_readlane(next_off, from) : 0;
+    const int page = ok ? entry : some_page;
+    const int use = page * a.block_size + (ok ? next_off : some_off);
     unsigned char* base = lds + stage * R::kStageB;
     if (lane == 0) flags[stage * kWaves + wave] = valid | zero << 16;
-    int r[R::kLoads];
+    uint32_t r[R::kLoads];
 #pragma unroll
     for (int i = 0; i < R::kLoads; ++i) r[i] = __shfl(use, i * R::kRowsPerLoad + lr, kWave);
     next_j += kBigTile;
     next_page += page_step;
     next_off += off_step;
-    if (next_off >= a.block_size) {
-      next_off -= a.block_size;
-      ++next_page;
-    }
-    load_entry();  // before the tile's own loads, which a wait for it leaves in flight
-    const float* scales = lane & 16 ? a.v_scales : a.k_scales;
-    load_lds4(scales + static_cast<int64_t>(page) * a.n_head_kv + kvh, base + 2 * R::kTileB + wave * kWave * 4);
+    const bool wrap = next_off >= a.block_size;
+    next_off -= wrap ? a.block_size : 0;
+    next_page += wrap ? 1 : 0;
+    load_entries();
+    load_lds4(scales_of + static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(a.n_head_kv),
+              base + 2 * R::kTileB + wave * kWave * 4);
 #pragma unroll
     for (int i = 0; i < R::kLoads; ++i) {
-      const int tr = wave * R::kWaveTileRows + i * R::kRowsPerLoad + lr;
+      const uint64_t off = static_cast<uint64_t>(r[i]) * row_b;
       const int at = (wave * R::kLoads + i) * 1024;
-      load_lds16(kp + r[i] * row_b + ((lc ^ k_place<D>(tr)) << 4), base + at);
-      load_lds16(vp + r[i] * row_b + ((lc ^ v_place32<D>(tr)) << 4), base + R::kTileB + at);
+      load_lds16(k_at[i] + off, base + at);
+      load_lds16(v_at[i] + off, base + R::kTileB + at);
     }
   };
 
@@ -767,17 +776,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
+  int nan_from = INT32_MAX, nan_to = 0;  // positions among which V codes that are NaN were left out
   if (n > 0) {
-    load_entry();
+    load_entries();
+    __builtin_amdgcn_s_waitcnt(wait_vm(0, true));
+    asm volatile("" ::: "memory");
     load_tile(0);
+    __builtin_amdgcn_s_waitcnt(wait_vm(R::kPerTile - 1, true));  // the entries, which went first
+    asm volatile("" ::: "memory");
     load_tile(1);  // past the end: rows that are not used
   }
   int stage = 0;
   for (int t = 0; t < n; ++t) {
-    // This wave's part of tile t is there (behind it: the next tile's loads
-    // and its table entry), and so is everyone's after the barrier, which no
-    // wave passes before all have read tile t - 1: its stage is free.
-    __builtin_amdgcn_s_waitcnt(wait_vm(R::kPerTile + 1, true));
+    // This wave's part of tile t is there, and the table entries of tile
+    // t + 2 (behind them: tile t + 1), and so is everyone's part after the
+    // barrier, which no wave passes before all have read tile t - 1: its
+    // stage is free.
+    __builtin_amdgcn_s_waitcnt(wait_vm(R::kPerTile - 1, true));
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
@@ -789,16 +804,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     stage = stage + 1 < kStages ? stage + 1 : 0;
     const int at = j0 + t * kBigTile;
     if (at >= wave_end) continue;  // none of this wave's rows
-    const uint64_t lo16 = (fl[0] & 0xFFFFu) | fl[1] << 16, hi16 = (fl[2] & 0xFFFFu) | fl[3] << 16;
-    const uint64_t valid = lo16 | hi16 << 32;
-    const uint64_t zero = static_cast<uint64_t>((fl[0] >> 16) | (fl[1] & 0xFFFF0000u)) |
-                          static_cast<uint64_t>((fl[2] >> 16) | (fl[3] & 0xFFFF0000u)) << 32;
-    const bool full = __builtin_amdgcn_readfirstlane(static_cast<int>(valid == ~0ull)) && at + kBigTile <= first_limit;
+    uint32_t fw[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) fw[w] = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[w]));
+    const bool full = (fw[0] & fw[1] & fw[2] & fw[3]) == 0xFFFFu && (fw[0] | fw[1] | fw[2] | fw[3]) == 0xFFFFu &&
+                      at + kBigTile <= first_limit;
     // Positions that this lane's row attends: rows of the pool, and rows of
     // zeros; bit 32 pt + 8 (i / 4) + i % 4 belongs to score i of sc[pt].
     uint32_t on[2] = {~0u, ~0u}, nil[2] = {0u, 0u};
     if (!full) {
       const uint64_t below = low_bits(limit - at);
+      const uint64_t valid = static_cast<uint64_t>((fw[0] & 0xFFFFu) | fw[1] << 16) |
+                             static_cast<uint64_t>((fw[2] & 0xFFFFu) | fw[3] << 16) << 32;
+      const uint64_t zero = static_cast<uint64_t>((fw[0] >> 16) | (fw[1] & 0xFFFF0000u)) |
+                            static_cast<uint64_t>((fw[2] >> 16) | (fw[3] & 0xFFFF0000u)) << 32;
       const uint64_t o = (valid & below) >> (4 * half), z = (zero & below) >> (4 * half);
       on[0] = static_cast<uint32_t>(o);
       on[1] = static_cast<uint32_t>(o >> 32);
@@ -811,11 +830,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     // multiply scores and weights.
     const float* k_of = scales + (col >> 4) * kWave + (col & 15);  // of position col of each 32
     const float ks[2] = {k_of[0], k_of[2 * kWave]};
-    const bool pow2 =
-        plan.aligned && !__any(!is_pow2(ks[0]) || !is_pow2(ks[1]) || !is_pow2(scales[(lane >> 4) * kWave + 16 + (lane & 15)]));
+    bool pow2 = plan.aligned;
+    if (pow2) {
+      const uint32_t x = __float_as_uint(ks[0]), y = __float_as_uint(ks[1]);
+      const uint32_t z = __float_as_uint(scales[(lane >> 4) * kWave + 16 + (lane & 15)]);
+      const bool odd = ((x | y | z) & 0x7FFFFFu) || min(min(x, y), z) < 0x800000u || max(max(x, y), z) >= 0x7F800000u;
+      pow2 = !__any(odd);
+    }
     float vs[8];  // of positions 8 g + 4 half + 0..3
 #pragma unroll
-    for (int g = 0; g < 8; ++g) vs[g] = pow2 ? scales[(g >> 1) * kWave + 16 + 8 * (g & 1) + 4 * half] : 1.f;
+    for (int g = 0; g < 8; ++g) vs[g] = 1.f;
+    if (pow2) {
+#pragma unroll
+      for (int g = 0; g < 8; ++g) vs[g] = scales[(g >> 1) * kWave + 16 + 8 * (g & 1) + 4 * half];
+    }
 
     // ---- scores
     f32x16_t sc[2];
@@ -857,6 +885,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[pt][i]);
     mx = max_halves(mx);
+    __builtin_amdgcn_sched_barrier(0);
+    // V's codes, asked for ahead of the softmax that hides their latency
+    u32x2_t v[4][D / 32];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = (lane & 15) >> 1, r = 16 * s + 8 * (k >> 2) + 4 * half + (k & 3);
+      const unsigned char* row = base + R::kTileB + r * D + 8 * (lane & 1);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+        v[s][d] = read_columns(row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4));
+    }
     __builtin_amdgcn_sched_barrier(0);
 
     // ---- softmax
@@ -912,47 +951,49 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     __builtin_amdgcn_sched_barrier(0);
 
     // ---- values
+    if (!full) {
+      uint32_t any = 0;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int k = (lane & 15) >> 1, r = 16 * s + 8 * (k >> 2) + 4 * half + (k & 3);
-      const unsigned char* row = base + R::kTileB + r * D + 8 * (lane & 1);
-      u32x2_t w[D / 32];
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-        w[d] = read_columns(row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4));
-      if (!full) {
-        uint32_t any = 0;
+        for (int d = 0; d < D / 32; ++d) any |= nan_bytes(v[s][d][0]) | nan_bytes(v[s][d][1]);
+      if (__builtin_expect(__any(any != 0), 0)) {
+        // for the rows that do not attend them: 0 * NaN is NaN; the others get theirs at the end
+        nan_from = min(nan_from, at);
+        nan_to = at + kBigTile;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) any |= nan_bytes(w[d][0]) | nan_bytes(w[d][1]);
-        if (__builtin_expect(__any(any != 0), 0)) {
-          float y[8];  // 1 where this lane's row attends the position
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = on[s / 2] & 1u << (8 * (2 * (s % 2) + e / 4) + e % 4) ? 1.f : 0.f;
-          u32x4_t one[1];
-          split8<1>(y, one);
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
           for (int d = 0; d < D / 32; ++d) {
-            const uint32_t n0 = (nan_bytes(w[d][0]) >> 7) * 0xFFu, n1 = (nan_bytes(w[d][1]) >> 7) * 0xFFu;
-            w[d][0] &= ~n0;
-            w[d][1] &= ~n1;
-            f32x16_t hit;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) hit[i] = 0.f;
-            hit = mfma32(f8x8_to_bf16x8(n0 & 0x38383838u, n1 & 0x38383838u), one[0], hit);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (hit[i] > 0.f) acc[d][i] = __builtin_nanf("");
+            v[s][d][0] &= ~((nan_bytes(v[s][d][0]) >> 7) * 0xFFu);
+            v[s][d][1] &= ~((nan_bytes(v[s][d][1]) >> 7) * 0xFFu);
           }
-        }
       }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
-        acc[d] = mfma32(scaled_bf16x8(w[d][0], vs[2 * s], w[d][1], vs[2 * s + 1]), p[s], acc[d]);
-    }
+        acc[d] = mfma32(scaled_bf16x8(v[s][d][0], vs[2 * s], v[s][d][1], vs[2 * s + 1]), p[s], acc[d]);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm(0, true));  // the loads past the end
 
-  // ---- this wave's rows: lane (half, col) holds dimensions 32 d + 8 i + 4 half + 0..3 of row col
+  // ---- this wave's rows: lane (half, col) holds dimensions 32 d + 8 i + 4 half + 0..3 of row col.
+  // V codes that are NaN, in the tiles where they were left out
+  for (int j = nan_from; j < min(nan_to, limit); ++j) {
+    const int lb = plan.block_div(j), pb = lb < a.max_blocks ? seq_table[lb] : -1;
+    if (pb < 0 || pb >= a.n_blocks) continue;
+    const uint8_t* row = vp + (static_cast<int64_t>(pb) * a.block_size + j - lb * a.block_size) * row_b + 4 * half;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t nan = nan_bytes(*reinterpret_cast<const uint32_t*>(row + 32 * d + 8 * g));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (nan >> (8 * i) & 0x80u) acc[d][4 * g + i] = __builtin_nanf("");
+      }
+  }
   l = sum_halves(l);
   if (token >= a.seq_len) return;
   const int64_t row = (static_cast<int64_t>(b) * a.seq_len + token) * a.n_head + head;
