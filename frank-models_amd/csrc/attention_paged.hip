@@ -30,6 +30,9 @@ __device__ __forceinline__ f32x4_t mfma16(const u32x4_t a, const u32x4_t b, f32x
 __device__ __forceinline__ void load_lds16(const void* src, void* dst) {
   __builtin_amdgcn_global_load_lds(src, dst, 16, 0, kNonTemporal);
 }
+__device__ __forceinline__ void load_lds16_cached(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
+}
 __device__ __forceinline__ void load_lds4(const void* src, void* dst) {
   __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0);
 }
@@ -586,8 +589,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 // (32x32x16) with A = V transposed, converted as it is read.
 constexpr int kBigRows = 128;
 constexpr int kWaveRows = 32;
-constexpr int kBigTile = 64;
-constexpr int kStages = 3;
+constexpr int kBigTile = 128;
+constexpr int kStages = 2;
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
 
@@ -624,8 +627,7 @@ struct Big {
   static constexpr int kTileB = kBigTile * D;
   static constexpr int kScaleB = kWaves * kWave * 4;
   static constexpr int kStageB = 2 * kTileB + kScaleB;
-  static constexpr int kLds = kStages * kStageB + kThreads * 4 + kStages * kWaves * 4;
-  static constexpr int kPerTile = 2 * kLoads + 2;  // loads per wave and tile, the entries of the next first
+  static constexpr int kLds = kStages * kStageB + kThreads * 4 + kStages * kWaves * 8;
   static constexpr int kWaveTileRows = kBigTile / kWaves;
   static_assert(kLoads * kRowsPerLoad == kWaveTileRows, "a wave loads whole rows");
 };
@@ -642,7 +644,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   using R = Big<D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int n_split = plan.n_split, split_len = plan.split_len;
-  uint32_t* flags = reinterpret_cast<uint32_t*>(lds + kStages * R::kStageB + kThreads * 4);  // [stage][wave]: valid, zero << 16
+  uint32_t* flags = reinterpret_cast<uint32_t*>(lds + kStages * R::kStageB + kThreads * 4);  // [stage]: valid by wave, zero by wave
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int half = lane >> 5, col = lane & 31;
@@ -672,11 +674,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   const uint8_t* kp = a.k_pool + kvh * D;
   const uint8_t* vp = a.v_pool + kvh * D;
 
-  // ---- loads.  Lanes l and l % 16 stand for position 16 wave + l % 16 of a
-  // tile.  All of them go to LDS, the table entries of a tile too, ahead of
-  // the loads of the tile before it: the compiler, which would wait for a
-  // register, leaves the counting to the waits below.
-  const int wp = wave * R::kWaveTileRows + (lane & 15);
+  // ---- loads.  Lanes l and l % 32 stand for position 32 wave + l % 32 of a
+  // tile.  All of them go to LDS, the table entries of the tile after it too,
+  // where the compiler does not wait for a register.
+  const int wp = wave * R::kWaveTileRows + (lane & 31);
   int next_j = j0 + wp, next_page = plan.block_div(next_j), next_off = next_j - next_page * a.block_size;
   const int page_step = plan.block_div(kBigTile), off_step = kBigTile - page_step * a.block_size;
   int* entries = reinterpret_cast<int*>(lds + kStages * R::kStageB) + wave * kWave;
@@ -684,28 +685,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     load_lds4(seq_table + min(next_page, a.max_blocks - 1), entries);
   };
   const int lr = lane / R::kPieces, lc = lane % R::kPieces;
-  const float* scales_of = (lane & 16 ? a.v_scales : a.k_scales) + kvh;
-  const uint8_t *k_at[R::kLoads], *v_at[R::kLoads];
+  const float* scales_of = (lane & 32 ? a.v_scales : a.k_scales) + kvh;
+  // The places of a wave's loads repeat every 16 rows.
+  constexpr int kPlaces = 16 / R::kRowsPerLoad;
+  const uint8_t *k_at[kPlaces], *v_at[kPlaces];
 #pragma unroll
-  for (int i = 0; i < R::kLoads; ++i) {
-    const int tr = wave * R::kWaveTileRows + i * R::kRowsPerLoad + lr;
-    k_at[i] = kp + ((lc ^ k_place<D>(tr)) << 4);
-    v_at[i] = vp + ((lc ^ v_place32<D>(tr)) << 4);
+  for (int i = 0; i < kPlaces; ++i) {
+    k_at[i] = kp + ((lc ^ k_place<D>(i * R::kRowsPerLoad + lr)) << 4);
+    v_at[i] = vp + ((lc ^ v_place32<D>(i * R::kRowsPerLoad + lr)) << 4);
   }
   auto load_tile = [&](int stage) __attribute__((always_inline)) {
     const int entry = entries[lane];
     const bool in = next_j < end;
     const bool ok = (next_page < a.max_blocks) & (static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.n_blocks)) & in;
-    const uint32_t valid = static_cast<uint32_t>(__ballot(ok)) & 0xFFFFu;
-    const uint32_t zero = static_cast<uint32_t>(__ballot(in & !ok)) & 0xFFFFu;
-    // unusable rows load a usable one (page 0 is there)
+    const uint32_t valid = static_cast<uint32_t>(__ballot(ok)), zero = static_cast<uint32_t>(__ballot(in & !ok));
+    // unusable rows load a usable one (row 0 is there)
     const int from = valid ? __builtin_ctz(valid) : 0;
     const int some_page = valid ? __builtin_amdgcn_readlane(entry, from) : 0;
     const int some_off = valid ? __builtin_amdgcn_readlane(next_off, from) : 0;
     const int page = ok ? entry : some_page;
     const int use = page * a.block_size + (ok ? next_off : some_off);
     unsigned char* base = lds + stage * R::kStageB;
-    if (lane == 0) flags[stage * kWaves + wave] = valid | zero << 16;
+    if (lane < 2) flags[stage * 2 * kWaves + kWaves * lane + wave] = lane ? zero : valid;
     uint32_t r[R::kLoads];
 #pragma unroll
     for (int i = 0; i < R::kLoads; ++i) r[i] = __shfl(use, i * R::kRowsPerLoad + lr, kWave);
@@ -722,8 +723,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     for (int i = 0; i < R::kLoads; ++i) {
       const uint64_t off = static_cast<uint64_t>(r[i]) * row_b;
       const int at = (wave * R::kLoads + i) * 1024;
-      load_lds16(k_at[i] + off, base + at);
-      load_lds16(v_at[i] + off, base + R::kTileB + at);
+      load_lds16_cached(k_at[i % kPlaces] + off, base + at);
+      load_lds16_cached(v_at[i % kPlaces] + off, base + R::kTileB + at);
     }
   };
 
@@ -782,201 +783,201 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     __builtin_amdgcn_s_waitcnt(wait_vm(0, true));
     asm volatile("" ::: "memory");
     load_tile(0);
-    __builtin_amdgcn_s_waitcnt(wait_vm(R::kPerTile - 1, true));  // the entries, which went first
-    asm volatile("" ::: "memory");
-    load_tile(1);  // past the end: rows that are not used
   }
-  int stage = 0;
   for (int t = 0; t < n; ++t) {
-    // This wave's part of tile t is there, and the table entries of tile
-    // t + 2 (behind them: tile t + 1), and so is everyone's part after the
-    // barrier, which no wave passes before all have read tile t - 1: its
-    // stage is free.
-    __builtin_amdgcn_s_waitcnt(wait_vm(R::kPerTile - 1, true));
+    // This wave's part of tile t is there, and the next tile's table entries,
+    // and so is everyone's part after the barrier, which no wave passes
+    // before all have read tile t - 1: its stage is free.
+    __builtin_amdgcn_s_waitcnt(wait_vm(0, true));
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
-    load_tile(stage >= 1 ? stage - 1 : kStages - 1);
-    const unsigned char* base = lds + stage * R::kStageB;
-    const float* scales = reinterpret_cast<const float*>(base + 2 * R::kTileB);
-    const u32x4_t fl = *reinterpret_cast<const u32x4_t*>(flags + stage * kWaves);
-    stage = stage + 1 < kStages ? stage + 1 : 0;
+    if (t + 1 < n) load_tile(~t & 1);
     const int at = j0 + t * kBigTile;
     if (at >= wave_end) continue;  // none of this wave's rows
-    uint32_t fw[4];
+    const unsigned char* base = lds + (t & 1) * R::kStageB;
+    const float* scales = reinterpret_cast<const float*>(base + 2 * R::kTileB);  // by wave: 32 of K, 32 of V
+    const uint32_t* fl = flags + (t & 1) * 2 * kWaves;
+    uint32_t valid[kWaves], all = ~0u;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) fw[w] = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[w]));
-    const bool full = (fw[0] & fw[1] & fw[2] & fw[3]) == 0xFFFFu && (fw[0] | fw[1] | fw[2] | fw[3]) == 0xFFFFu &&
-                      at + kBigTile <= first_limit;
-    // Positions that this lane's row attends: rows of the pool, and rows of
-    // zeros; bit 32 pt + 8 (i / 4) + i % 4 belongs to score i of sc[pt].
-    uint32_t on[2] = {~0u, ~0u}, nil[2] = {0u, 0u};
-    if (!full) {
-      const uint64_t below = low_bits(limit - at);
-      const uint64_t valid = static_cast<uint64_t>((fw[0] & 0xFFFFu) | fw[1] << 16) |
-                             static_cast<uint64_t>((fw[2] & 0xFFFFu) | fw[3] << 16) << 32;
-      const uint64_t zero = static_cast<uint64_t>((fw[0] >> 16) | (fw[1] & 0xFFFF0000u)) |
-                            static_cast<uint64_t>((fw[2] >> 16) | (fw[3] & 0xFFFF0000u)) << 32;
-      const uint64_t o = (valid & below) >> (4 * half), z = (zero & below) >> (4 * half);
-      on[0] = static_cast<uint32_t>(o);
-      on[1] = static_cast<uint32_t>(o >> 32);
-      nil[0] = static_cast<uint32_t>(z);
-      nil[1] = static_cast<uint32_t>(z >> 32);
+    for (int w = 0; w < kWaves; ++w) {
+      valid[w] = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[w]));
+      all &= valid[w];
     }
-
-    // Scales that are powers of two, one for four neighbouring positions, cost
-    // nothing: the products take K's, the conversion of V takes V's.  Others
-    // multiply scores and weights.
-    const float* k_of = scales + (col >> 4) * kWave + (col & 15);  // of position col of each 32
-    const float ks[2] = {k_of[0], k_of[2 * kWave]};
+    const bool full = all == ~0u && at + kBigTile <= first_limit;
+    // Scales that are powers of two, V's one for four neighbouring positions,
+    // cost nothing: the products take K's, the conversion of V takes V's.
+    // Others multiply scores and weights.
+    float ks[kWaves];  // of position col of each 32
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) ks[w] = scales[w * kWave + col];
     bool pow2 = plan.aligned;
     if (pow2) {
-      const uint32_t x = __float_as_uint(ks[0]), y = __float_as_uint(ks[1]);
-      const uint32_t z = __float_as_uint(scales[(lane >> 4) * kWave + 16 + (lane & 15)]);
-      const bool odd = ((x | y | z) & 0x7FFFFFu) || min(min(x, y), z) < 0x800000u || max(max(x, y), z) >= 0x7F800000u;
-      pow2 = !__any(odd);
-    }
-    float vs[8];  // of positions 8 g + 4 half + 0..3
+      uint32_t any = 0, least = ~0u, most = 0;
 #pragma unroll
-    for (int g = 0; g < 8; ++g) vs[g] = 1.f;
-    if (pow2) {
-#pragma unroll
-      for (int g = 0; g < 8; ++g) vs[g] = scales[(g >> 1) * kWave + 16 + 8 * (g & 1) + 4 * half];
-    }
-
-    // ---- scores
-    f32x16_t sc[2];
-#pragma unroll
-    for (int pt = 0; pt < 2; ++pt) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[pt][i] = 0.f;
-      const int r = 32 * pt + col;
-      const int e8m0 = pow2 ? static_cast<int>(__float_as_uint(ks[pt]) >> 23) : 127;
-#pragma unroll
-      for (int s = 0; s < D / 64; ++s) {
-        u32x4_t w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          w[e] = *reinterpret_cast<const u32x4_t*>(base + r * D + (((4 * s + 2 * half + e) ^ k_place<D>(r)) << 4));
-        const i32x8_t k = __builtin_bit_cast(i32x8_t, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        sc[pt] = mfma32_f8(k, e8m0, qh[s], sc[pt]);
-        sc[pt] = mfma32_f8(k, e8m0, ql[s], sc[pt]);
+      for (int w = 0; w < kWaves; ++w) {
+        const uint32_t u = __float_as_uint(scales[w * kWave + lane]);
+        any |= u;
+        least = min(least, u);
+        most = max(most, u);
       }
+      pow2 = !__any((any & 0x7FFFFFu) | (least < 0x800000u) | (most >= 0x7F800000u));
     }
-    if (!pow2) {
 #pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
+    for (int h64 = 0; h64 < 2; ++h64) {  // 64 positions at a time
+      const int half_at = at + 64 * h64;
+      if (half_at >= wave_end) break;
+      float vs[8];  // of positions 8 g + 4 half + 0..3
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[pt][i] *= scales[(2 * pt + (i >> 3)) * kWave + 8 * (i >> 2 & 1) + 4 * half + (i & 3)];
-    }
-    if (!full) {
+      for (int g = 0; g < 8; ++g) vs[g] = 1.f;
+      if (pow2) {
 #pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
+        for (int g = 0; g < 8; ++g) vs[g] = scales[(2 * h64 + (g >> 2)) * kWave + 32 + 8 * (g & 3) + 4 * half];
+      }
+      // Positions that this lane's row attends: rows of the pool, and rows of
+      // zeros; bit 8 (i / 4) + i % 4 of word pt belongs to score i of sc[pt].
+      uint32_t on[2] = {~0u, ~0u}, nil[2] = {0u, 0u};
+      if (!full) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t bit = 1u << (8 * (i >> 2) + (i & 3));
-          sc[pt][i] = on[pt] & bit ? sc[pt][i] : nil[pt] & bit ? 0.f : -INFINITY;
+        for (int pt = 0; pt < 2; ++pt) {
+          const uint32_t below = static_cast<uint32_t>(low_bits(min(limit - half_at - 32 * pt, 32)));
+          on[pt] = (valid[2 * h64 + pt] & below) >> (4 * half);
+          nil[pt] = (fl[kWaves + 2 * h64 + pt] & below) >> (4 * half);
         }
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[pt][i]);
-    mx = max_halves(mx);
-    __builtin_amdgcn_sched_barrier(0);
-    // V's codes, asked for ahead of the softmax that hides their latency
-    u32x2_t v[4][D / 32];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int k = (lane & 15) >> 1, r = 16 * s + 8 * (k >> 2) + 4 * half + (k & 3);
-      const unsigned char* row = base + R::kTileB + r * D + 8 * (lane & 1);
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-        v[s][d] = read_columns(row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4));
-    }
-    __builtin_amdgcn_sched_barrier(0);
+      }
 
-    // ---- softmax
-    if (__any((mx - m) * c2 > kLazy)) {
-      const float top = fmaxf(m, mx);
-      const float f = __builtin_amdgcn_exp2f((m - finite_base(top)) * c2);
-      m = top;
-      l *= f;
+      // ---- scores
+      f32x16_t sc[2];
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d)
+      for (int pt = 0; pt < 2; ++pt) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[d][i] *= f;
-    }
-    const float mc = finite_base(m) * c2;
-    u32x4_t p[4];
+        for (int i = 0; i < 16; ++i) sc[pt][i] = 0.f;
+        const int r = 64 * h64 + 32 * pt + col;
+        const int e8m0 = pow2 ? static_cast<int>(__float_as_uint(ks[2 * h64 + pt]) >> 23) : 127;
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt) {
-      float w[16];
+        for (int s = 0; s < D / 64; ++s) {
+          u32x4_t w[2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(sc[pt][i], c2, -mc));
+          for (int e = 0; e < 2; ++e)
+            w[e] = *reinterpret_cast<const u32x4_t*>(base + r * D + (((4 * s + 2 * half + e) ^ k_place<D>(r)) << 4));
+          const i32x8_t k = __builtin_bit_cast(i32x8_t, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          sc[pt] = mfma32_f8(k, e8m0, qh[s], sc[pt]);
+          sc[pt] = mfma32_f8(k, e8m0, ql[s], sc[pt]);
+        }
+      }
       if (!pow2) {
-        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sum += w[i];
-          w[i] *= scales[(2 * pt + (i >> 3)) * kWave + 16 + 8 * (i >> 2 & 1) + 4 * half + (i & 3)];
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[pt][i] *= scales[(2 * h64 + pt) * kWave + 8 * (i >> 2) + 4 * half + (i & 3)];
+      }
+      if (!full) {
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t bit = 1u << (8 * (i >> 2) + (i & 3));
+            sc[pt][i] = on[pt] & bit ? sc[pt][i] : nil[pt] & bit ? 0.f : -INFINITY;
+          }
+      }
+      float top4[4];  // four chains
+#pragma unroll
+      for (int g = 0; g < 4; ++g) top4[g] = sc[g >> 1][8 * (g & 1)];
+#pragma unroll
+      for (int i = 1; i < 8; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) top4[g] = fmaxf(top4[g], sc[g >> 1][8 * (g & 1) + i]);
+      const float mx = max_halves(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
+      __builtin_amdgcn_sched_barrier(0);
+      // V's codes, asked for ahead of the softmax that hides their latency
+      u32x2_t v[4][D / 32];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int k = (lane & 15) >> 1, r = 64 * h64 + 16 * s + 8 * (k >> 2) + 4 * half + (k & 3);
+        const unsigned char* row = base + R::kTileB + r * D + 8 * (lane & 1);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          v[s][d] = read_columns(row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
+      // ---- softmax
+      if (__any((mx - m) * c2 > kLazy)) {
+        const float top = fmaxf(m, mx);
+        const float f = __builtin_amdgcn_exp2f((m - finite_base(top)) * c2);
+        m = top;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+      }
+      const float mc = finite_base(m) * c2;
+      u32x4_t p[4];
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt) {
+        float w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(sc[pt][i], c2, -mc));
+        if (!pow2) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sums[i & 3] += w[i];
+            w[i] *= scales[(2 * h64 + pt) * kWave + 32 + 8 * (i >> 2) + 4 * half + (i & 3)];
+            if (!(on[pt] & 1u << (8 * (i >> 2) + (i & 3)))) w[i] = 0.f;  // 0 times a scale that is not finite
+          }
         }
-        l += sum;
-      }
-      if (!full && !pow2) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (!(on[pt] & 1u << (8 * (i >> 2) + (i & 3)))) w[i] = 0.f;  // 0 times a scale that is not finite
-      }
-      split8<1>(w, &p[2 * pt]);
-      split8<1>(w + 8, &p[2 * pt + 1]);
-      if (pow2) {  // the sum of the weights as they are multiplied, rounded to bf16
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) l = add_bf16x2(p[2 * pt + g][e], l);
-        if (!full) {  // a row of zeros has its weight and no value
+        split8<1>(w, &p[2 * pt]);
+        split8<1>(w + 8, &p[2 * pt + 1]);
+        if (pow2) {  // the sum of the weights as they are multiplied, rounded to bf16
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t bits = on[pt] >> (8 * (2 * g + (e >> 1)) + 2 * (e & 1));
-              p[2 * pt + g][e] &= (bits & 1 ? 0xFFFFu : 0u) | (bits & 2 ? 0xFFFF0000u : 0u);
-            }
+            for (int e = 0; e < 4; ++e) sums[e] = add_bf16x2(p[2 * pt + g][e], sums[e]);
+          if (!full) {  // a row of zeros has its weight and no value
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t bits = on[pt] >> (8 * (2 * g + (e >> 1)) + 2 * (e & 1));
+                p[2 * pt + g][e] &= (bits & 1 ? 0xFFFFu : 0u) | (bits & 2 ? 0xFFFF0000u : 0u);
+              }
+          }
         }
       }
-    }
-    __builtin_amdgcn_sched_barrier(0);
+      l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      __builtin_amdgcn_sched_barrier(0);
 
-    // ---- values
-    if (!full) {
-      uint32_t any = 0;
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) any |= nan_bytes(v[s][d][0]) | nan_bytes(v[s][d][1]);
-      if (__builtin_expect(__any(any != 0), 0)) {
-        // for the rows that do not attend them: 0 * NaN is NaN; the others get theirs at the end
-        nan_from = min(nan_from, at);
-        nan_to = at + kBigTile;
+      // ---- values
+      if (!full) {
+        uint32_t any = 0;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d) {
-            v[s][d][0] &= ~((nan_bytes(v[s][d][0]) >> 7) * 0xFFu);
-            v[s][d][1] &= ~((nan_bytes(v[s][d][1]) >> 7) * 0xFFu);
-          }
+          for (int d = 0; d < D / 32; ++d) any |= nan_bytes(v[s][d][0]) | nan_bytes(v[s][d][1]);
+        if (__builtin_expect(__any(any != 0), 0)) {
+          // for the rows that do not attend them: 0 * NaN is NaN; the others get theirs at the end
+          nan_from = min(nan_from, half_at);
+          nan_to = half_at + 64;
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+              v[s][d][0] &= ~((nan_bytes(v[s][d][0]) >> 7) * 0xFFu);
+              v[s][d][1] &= ~((nan_bytes(v[s][d][1]) >> 7) * 0xFFu);
+            }
+        }
       }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          acc[d] = mfma32(scaled_bf16x8(v[s][d][0], vs[2 * s], v[s][d][1], vs[2 * s + 1]), p[s], acc[d]);
     }
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-        acc[d] = mfma32(scaled_bf16x8(v[s][d][0], vs[2 * s], v[s][d][1], vs[2 * s + 1]), p[s], acc[d]);
   }
-  __builtin_amdgcn_s_waitcnt(wait_vm(0, true));  // the loads past the end
+  __builtin_amdgcn_s_waitcnt(wait_vm(0, true));  // the entries past the end
 
   // ---- this wave's rows: lane (half, col) holds dimensions 32 d + 8 i + 4 half + 0..3 of row col.
   // V codes that are NaN, in the tiles where they were left out
@@ -1132,7 +1133,7 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
     p.waves_per_tile = 1;
     blocks = pairs * ((rows + kBigRows - 1) / kBigRows);
     n = 512 / blocks;
-    step = 4 * kBigTile;
+    step = 2 * kBigTile;
   } else {
     // About 1024 waves, one per SIMD, which keep the memory as busy as twice
     // as many (64 x 8192 positions 176 against 171 us) and spend half the
