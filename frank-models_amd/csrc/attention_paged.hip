@@ -39,12 +39,75 @@ __device__ __forceinline__ void load_lds4(const void* src, void* dst) {
 
 // Eight codes of one column from eight rows of a tile in LDS: the lanes
 // 2k and 2k + 1 of a group of 16 name row k's 8 low and 8 high columns, and
-// lane c of the group gets column c, row k in byte k.
-__device__ __forceinline__ u32x2_t read_columns(const unsigned char* p) {
-  typedef __attribute__((ext_vector_type(2))) int i32x2_t;
-  const auto v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-      (__attribute__((address_space(3))) i32x2_t*)(__attribute__((address_space(3))) void*)p);
-  return __builtin_bit_cast(u32x2_t, v);
+// lane c of the group gets column c, row k in byte k.  Several at once and
+// waited for together, in assembly: before the compiler's own reads of this
+// kind it waits for every load to LDS in flight, the next tiles' too, which
+// took a decode step of 64 x 8192 positions from 176 to TBD us.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
+}
+
+template <int N>
+__device__ __forceinline__ void read_columns(const uint32_t (&at)[N], u32x2_t (&w)[N]) {
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "one column piece per 16 dimensions");
+  if constexpr (N == 1) {
+    asm volatile("ds_read_b64_tr_b8 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(w[0]) : "v"(at[0]) : "memory");
+  } else if constexpr (N == 2) {
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %2\n\tds_read_b64_tr_b8 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1])
+        : "v"(at[0]), "v"(at[1])
+        : "memory");
+  } else if constexpr (N == 4) {
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\t"
+        "ds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %9\n\t"
+        "ds_read_b64_tr_b8 %2, %10\n\tds_read_b64_tr_b8 %3, %11\n\t"
+        "ds_read_b64_tr_b8 %4, %12\n\tds_read_b64_tr_b8 %5, %13\n\t"
+        "ds_read_b64_tr_b8 %6, %14\n\tds_read_b64_tr_b8 %7, %15\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7])
+        : "memory");
+  }
+}
+
+// The same for four steps of kStep bytes from each address.
+template <int kStep, int N>
+__device__ __forceinline__ void read_columns4(const uint32_t (&at)[N], u32x2_t (&w)[4][N]) {
+  static_assert(N == 2 || N == 4, "32 columns each");
+  if constexpr (N == 2) {
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %9\n\t"
+        "ds_read_b64_tr_b8 %2, %8 offset:%10\n\tds_read_b64_tr_b8 %3, %9 offset:%10\n\t"
+        "ds_read_b64_tr_b8 %4, %8 offset:%11\n\tds_read_b64_tr_b8 %5, %9 offset:%11\n\t"
+        "ds_read_b64_tr_b8 %6, %8 offset:%12\n\tds_read_b64_tr_b8 %7, %9 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1]), "=&v"(w[2][0]), "=&v"(w[2][1]),
+          "=&v"(w[3][0]), "=&v"(w[3][1])
+        : "v"(at[0]), "v"(at[1]), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %16\n\tds_read_b64_tr_b8 %1, %17\n\t"
+        "ds_read_b64_tr_b8 %2, %18\n\tds_read_b64_tr_b8 %3, %19\n\t"
+        "ds_read_b64_tr_b8 %4, %16 offset:%20\n\tds_read_b64_tr_b8 %5, %17 offset:%20\n\t"
+        "ds_read_b64_tr_b8 %6, %18 offset:%20\n\tds_read_b64_tr_b8 %7, %19 offset:%20\n\t"
+        "ds_read_b64_tr_b8 %8, %16 offset:%21\n\tds_read_b64_tr_b8 %9, %17 offset:%21\n\t"
+        "ds_read_b64_tr_b8 %10, %18 offset:%21\n\tds_read_b64_tr_b8 %11, %19 offset:%21\n\t"
+        "ds_read_b64_tr_b8 %12, %16 offset:%22\n\tds_read_b64_tr_b8 %13, %17 offset:%22\n\t"
+        "ds_read_b64_tr_b8 %14, %18 offset:%22\n\tds_read_b64_tr_b8 %15, %19 offset:%22\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[0][2]), "=&v"(w[0][3]), "=&v"(w[1][0]), "=&v"(w[1][1]),
+          "=&v"(w[1][2]), "=&v"(w[1][3]), "=&v"(w[2][0]), "=&v"(w[2][1]), "=&v"(w[2][2]), "=&v"(w[2][3]),
+          "=&v"(w[3][0]), "=&v"(w[3][1]), "=&v"(w[3][2]), "=&v"(w[3][3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep)
+        : "memory");
+  }
 }
 
 // 0x80 in each byte that is a NaN code (0x7F, 0xFF).
@@ -481,9 +544,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 #pragma unroll
       for (int g = 0; g < kPg; ++g) {
         const int k = (lane & 15) >> 1, r = 16 * (k >> 2) + 4 * q4 + (k & 3);
-        const unsigned char* tile = ring + (kT + it) * R::kTileB + (32 * g + r) * D + 8 * (lane & 1);
+        const uint32_t tile = lds_address(ring + (kT + it) * R::kTileB + (32 * g + r) * D + 8 * (lane & 1));
+        uint32_t from[D / 16];
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) w[g][t] = read_columns(tile + ((t ^ v_place<D>(r)) << 4));
+        for (int t = 0; t < D / 16; ++t) from[t] = tile + ((t ^ v_place<D>(r)) << 4);
+        read_columns(from, w[g]);
       }
       __builtin_amdgcn_s_waitcnt(wait_vm(63, true));
       __builtin_amdgcn_sched_barrier(0);
@@ -890,18 +955,6 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
         for (int g = 0; g < 4; ++g) top4[g] = fmaxf(top4[g], sc[g >> 1][8 * (g & 1) + i]);
       const float mx = max_halves(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
       __builtin_amdgcn_sched_barrier(0);
-      // V's codes, asked for ahead of the softmax that hides their latency
-      u32x2_t v[4][D / 32];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = (lane & 15) >> 1, r = 64 * h64 + 16 * s + 8 * (k >> 2) + 4 * half + (k & 3);
-        const unsigned char* row = base + R::kTileB + r * D + 8 * (lane & 1);
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          v[s][d] = read_columns(row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-
       // ---- softmax
       if (__any((mx - m) * c2 > kLazy)) {
         const float top = fmaxf(m, mx);
@@ -951,6 +1004,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
       __builtin_amdgcn_sched_barrier(0);
 
       // ---- values
+      u32x2_t v[4][D / 32];
+      {
+        const int k = (lane & 15) >> 1, r = 64 * h64 + 8 * (k >> 2) + 4 * half + (k & 3);  // and 16 s
+        const uint32_t row = lds_address(base + R::kTileB + r * D + 8 * (lane & 1));
+        uint32_t from[D / 32];
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) from[d] = row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4);
+        read_columns4<16 * D>(from, v);
+      }
       if (!full) {
         uint32_t any = 0;
 #pragma unroll
@@ -1119,20 +1181,30 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, P
 
 // Which kernel, and how the context is cut: for two blocks per CU where the
 // rows alone do not give them.
-constexpr int kBigFrom = 64;  // query rows of a K/V head
+// The kernel for many rows where (row, position) pairs are at least 12 M and a
+// K/V head has 32 rows: below, most of its 128-row blocks' time is latency,
+// and the other's 16-row tiles fill the GPU (4 query heads x 128, 8 K/V heads;
+// few rows against many rows: 512 tokens of 512 16.6 against 27.4 us, 128 of 2048
+// 26.5 and 27.7, 64 of 8192 44.1 and 35.7, 8 x 256 of 256 35.0 and 22.2, 8 x 8
+// of 8192 51.6 and 46.4).
+constexpr int64_t kBigPairs = 12ll << 20;
+constexpr int kBigFrom = 32;
 
 Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int block_size, int q_dtype) {
   const int64_t rows = static_cast<int64_t>(seq_len) * (n_head / n_head_kv);
   const int64_t pairs = static_cast<int64_t>(batch) * n_head_kv;
   Plan p;
   p.aligned = block_size % 4 == 0;
-  p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom;
+  p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom && pairs * rows * max_ctx >= kBigPairs;
   int64_t blocks, n;
   int step;
   if (p.big) {
     p.waves_per_tile = 1;
     blocks = pairs * ((rows + kBigRows - 1) / kBigRows);
     n = 512 / blocks;
+    // Two splits of causal prompts are not worth joining (1024 tokens of 1024:
+    // 48 against 38 us with one).
+    if (n == 2 && max_ctx < 4ll * seq_len) n = 1;
     step = 2 * kBigTile;
   } else {
     // About 1024 waves, one per SIMD, which keep the memory as busy as twice
