@@ -1187,7 +1187,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, P
 // few rows against many rows: 512 tokens of 512 16.6 against 27.4 us, 128 of 2048
 // 26.5 and 27.7, 64 of 8192 44.1 and 35.7, 8 x 256 of 256 35.0 and 22.2, 8 x 8
 // of 8192 51.6 and 46.4).
-constexpr int64_t kBigPairs = 12ll << 20;
+constexpr double kBigPairs = 12 << 20;
 constexpr int kBigFrom = 32;
 
 Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int block_size, int q_dtype) {
@@ -1195,7 +1195,7 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
   const int64_t pairs = static_cast<int64_t>(batch) * n_head_kv;
   Plan p;
   p.aligned = block_size % 4 == 0;
-  p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom && pairs * rows * max_ctx >= kBigPairs;
+  p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom && static_cast<double>(pairs) * rows * max_ctx >= kBigPairs;
   int64_t blocks, n;
   int step;
   if (p.big) {

@@ -366,6 +366,73 @@ def test_queries_that_are_not_finite_stay_in_their_rows(fm):
         assert torch.equal(bad[0][keep], good[0][keep])
 
 
+# ---------------------------------------------------------------- many rows
+def many(B, S, H, context):
+    """A max_context_len for which the call is one of many (row, position)
+    pairs, whatever the contexts: the kernel is chosen by it."""
+    return max(max(context), (16 << 20) // (B * S * H))
+
+
+@pytest.mark.parametrize("pow2", [True, False])
+@pytest.mark.parametrize("B,S,H,Hkv,D,bs,context,lens,causal", [
+    (2, 32, 1, 1, 128, 16, [32, 77], None, True),
+    (3, 33, 4, 1, 128, 16, [33, 64, 31], [33, 20, 33], True),  # a context shorter than its tokens
+    (2, 64, 2, 2, 64, 32, [64, 200], [64, 63], True),
+    (2, 130, 4, 1, 128, 16, [130, 257], [130, 129], True),
+    (1, 257, 3, 1, 128, 100, [257], None, True),
+    (2, 66, 8, 4, 128, 4, [200, 66], [66, 1], False),
+    (2, 40, 4, 2, 64, 5, [130, 90], [40, 0], False),
+    (1, 70, 20, 2, 64, 1, [515], None, True),
+    (3, 48, 6, 2, 128, 64, [48, 640, 1000], [48, 16, 3], True),
+])
+def test_many_rows(fm, pow2, B, S, H, Hkv, D, bs, context, lens, causal, monkeypatch):
+    """Row tiles of 128 at their edges, scales that are powers of two and not."""
+    rng = np.random.default_rng(B * S + D + bs)
+    if pow2:
+        pool = random_pool
+        monkeypatch.setattr(__import__(__name__), "random_pool",
+                            lambda *a: (lambda c, s: (c, np.exp2(np.round(np.log2(s))).astype(np.float32)))(*pool(*a)))
+    check_attention(fm, rng, "bf16", B, S, H, Hkv, D, bs, context, lens, causal, wide=S % 2 == 1,
+                    max_context=many(B, S, H, context))
+
+
+@pytest.mark.parametrize("B,S,H,Hkv,D,context", [(1, 100, 8, 2, 128, 3001), (2, 200, 4, 1, 64, 1500), (9, 256, 32, 4, 128, 300)])
+def test_many_rows_long_contexts(fm, B, S, H, Hkv, D, context):
+    rng = np.random.default_rng(S)
+    contexts = [context - 7 * b for b in range(B)]
+    check_attention(fm, rng, "bf16", B, S, H, Hkv, D, 16, contexts, None,
+                    max_context=max(context, (13 << 20) // (B * S * H)))
+
+
+def test_many_rows_bad_pages_and_cut_contexts(fm):
+    rng = np.random.default_rng(21)
+    S, H = 150, 4
+    table = rng.permutation(40).reshape(2, 20)
+    table[0, 3], table[0, 7], table[1, 0], table[1, 19] = -1, 40, 1 << 30, -(1 << 31)
+    table[1, 8:16] = 77  # a whole tile of zeros
+    for causal in (True, False):
+        check_attention(fm, rng, "bf16", 2, S, H, 1, 128, 16, [320, 330], None, causal, table=table, n_blocks=40,
+                        max_context=16 << 15)
+        check_attention(fm, rng, "bf16", 2, S, H, 1, 64, 16, [16 << 15, 300], None, causal, 0.5, table=table,
+                        n_blocks=40, max_context=16 << 10)
+
+
+@pytest.mark.parametrize("S,D,bs", [(40, 64, 16), (70, 128, 16), (140, 128, 64), (33, 128, 3)])
+def test_many_rows_what_is_masked_has_no_influence(fm, S, D, bs, monkeypatch):
+    real = fm.attention_paged
+    monkeypatch.setattr(fm, "attention_paged",
+                        lambda q, k, v, layer, bt, cl, n, **kw: real(q, k, v, layer, bt, cl, 16 << 15, **kw))
+    test_what_is_masked_has_no_influence(fm, "bf16", S, D, bs)
+
+
+def test_many_rows_extreme_sizes_and_queries(fm, monkeypatch):
+    real = fm.attention_paged
+    monkeypatch.setattr(fm, "attention_paged",
+                        lambda q, k, v, layer, bt, cl, n, **kw: real(q, k, v, layer, bt, cl, 16 << 16, **kw))
+    test_scores_and_weights_of_extreme_size(fm, "bf16", 90)
+    test_queries_that_are_not_finite_stay_in_their_rows(fm)
+
+
 # ---------------------------------------------------------------- a run of both
 @pytest.mark.parametrize("act", ["bf16", "f32"])
 def test_prompt_then_decode(fm, act):
