@@ -20,6 +20,7 @@ import torch
 
 from . import _lib as L
 from .api import _DT_TO_TORCH, _TORCH_TO_DT, _device, _dtype_code, _finish, _ptr, _stream, _to_device, _workspace
+from .kvpool import QuantizedKVPool, check_pools, here
 
 
 def _ints_to_device(a, name: str, dtype=torch.int32) -> torch.Tensor:
@@ -177,9 +178,10 @@ class AttentionBlockDecode:
         self.head_dim = self.n_embd // self.n_head
         self._ws = None
 
-    def _get_ws(self, batch, ctx, sublayer=False):
-        fn = ("fmoe_attention_sublayer_decode_paged_workspace_bytes" if sublayer
-              else "fmoe_attention_block_decode_workspace_bytes")
+    def _get_ws(self, batch, ctx, sublayer=False, codes=False):
+        f8 = "_f8" if codes else ""
+        fn = (f"fmoe_attention_sublayer_decode_paged{f8}_workspace_bytes" if sublayer
+              else f"fmoe_attention_decode_paged{f8}_workspace_bytes")
         nbytes = getattr(L.lib(), fn)(batch, ctx, self.n_head, self.n_head_kv, self.n_embd, self.n_embd_kv, self.act)
         dev = torch.device("cuda", torch.cuda.current_device())
         if self._ws is None or self._ws.numel() < nbytes or self._ws.device != dev:
@@ -223,8 +225,13 @@ class AttentionBlockDecode:
     def _paged_args(self, B, dt, k_cache, v_cache, block_tables, context_lens, block_indices, pos_in_blocks):
         """Checks the pools and paging metadata of a paged call; returns the
         device int32 tensors (tables, lens, block indices, positions in block)."""
+        quantized = isinstance(k_cache, QuantizedKVPool) or isinstance(v_cache, QuantizedKVPool)
+        if quantized:
+            check_pools(k_cache, v_cache, here())
         for name, p in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if not isinstance(p, torch.Tensor) or p.dtype != dt or p.device.type != "cuda" or not p.is_contiguous():
+            p = p.data if quantized else p
+            if not quantized and (not isinstance(p, torch.Tensor) or p.dtype != dt or p.device.type != "cuda"
+                                  or not p.is_contiguous()):
                 raise TypeError(f"{name} must be a contiguous {dt} device tensor")
             if p.dim() != 4 or tuple(p.shape[2:]) != (self.n_head_kv, self.head_dim):
                 raise ValueError(f"{name} must be [n_blocks, block_size, {self.n_head_kv}, {self.head_dim}]")
@@ -240,8 +247,11 @@ class AttentionBlockDecode:
 
     def _paging(self, k_cache, v_cache, layer, bt, cl, max_context_len, bi, pi):
         """The C ABI's pool and paging arguments, from k_cache to pos_in_blocks."""
-        return (_ptr(k_cache), _ptr(v_cache), int(k_cache.shape[0]), int(k_cache.shape[1]), int(layer), _ptr(bt),
-                _ptr(cl), int(bt.shape[0]), int(bt.shape[2]), int(max_context_len), _ptr(bi), _ptr(pi))
+        pools = (k_cache, v_cache)
+        if isinstance(k_cache, QuantizedKVPool):
+            pools = (k_cache.data, v_cache.data, k_cache.scales, v_cache.scales)
+        return (*map(_ptr, pools), int(k_cache.shape[0]), int(k_cache.shape[1]), int(layer), _ptr(bt), _ptr(cl),
+                int(bt.shape[0]), int(bt.shape[2]), int(max_context_len), _ptr(bi), _ptr(pi))
 
     def _tail(self, B, out, k_new, v_new, ws):
         return (B, self.n_head, self.n_head_kv, self.n_embd, self.n_embd_kv, self.freq_base, self.freq_scale,
@@ -251,7 +261,13 @@ class AttentionBlockDecode:
               block_indices, pos_in_blocks):
         """Attention of one new token per sequence over the paged pools
         ``[n_blocks, block_size, n_head_kv, head_dim]`` (updated in place with
-        the new K/V) -> ``(out, k_new, v_new)``."""
+        the new K/V) -> ``(out, k_new, v_new)``.
+
+        With two ``QuantizedKVPool``s the query, rounded to ``x``'s type,
+        attends their codes, and its own key and value as they were projected.
+        ``kvcache_append``'s rules hold for what is written: of slots in one
+        page, which sequences with pages of their own never name, the last
+        sequence's alone."""
         x, pos = self._x(x, positions)
         B, dt = int(x.shape[0]), x.dtype
         bt, cl, bi, pi = self._paged_args(B, dt, k_cache, v_cache, block_tables, context_lens, block_indices,
@@ -259,8 +275,9 @@ class AttentionBlockDecode:
         out = torch.empty((B, self.n_embd), dtype=dt, device=x.device)
         k_new = torch.empty((B, self.n_head_kv, self.head_dim), dtype=dt, device=x.device)
         v_new = torch.empty_like(k_new)
-        ws = self._get_ws(B, int(max_context_len))
-        L.call("fmoe_attention_decode_paged", _ptr(x), _ptr(pos),
+        codes = isinstance(k_cache, QuantizedKVPool)
+        ws = self._get_ws(B, int(max_context_len), codes=codes)
+        L.call("fmoe_attention_decode_paged_f8" if codes else "fmoe_attention_decode_paged", _ptr(x), _ptr(pos),
                *self._paging(k_cache, v_cache, layer, bt, cl, max_context_len, bi, pi), *self._weights(),
                *self._tail(B, out, k_new, v_new, ws))
         return out, k_new, v_new
@@ -285,8 +302,9 @@ class AttentionBlockDecode:
             raise ValueError(f"out must be a contiguous {dt} [{B}, {self.n_embd}] tensor")
         k_new = torch.empty((B, self.n_head_kv, self.head_dim), dtype=dt, device=x.device)
         v_new = torch.empty_like(k_new)
-        ws = self._get_ws(B, int(max_context_len), sublayer=True)
-        L.call("fmoe_attention_sublayer_decode_paged", _ptr(x), _ptr(nw), float(rms_eps), _ptr(pos),
+        codes = isinstance(k_cache, QuantizedKVPool)
+        ws = self._get_ws(B, int(max_context_len), sublayer=True, codes=codes)
+        L.call("fmoe_attention_sublayer_decode_paged_f8" if codes else "fmoe_attention_sublayer_decode_paged", _ptr(x), _ptr(nw), float(rms_eps), _ptr(pos),
                *self._paging(k_cache, v_cache, layer, bt, cl, max_context_len, bi, pi), *self._weights(),
                *self._tail(B, out, k_new, v_new, ws))
         return out, k_new, v_new

@@ -42,7 +42,7 @@ __device__ __forceinline__ void load_lds4(const void* src, void* dst) {
 // lane c of the group gets column c, row k in byte k.  Several at once and
 // waited for together, in assembly: before the compiler's own reads of this
 // kind it waits for every load to LDS in flight, the next tiles' too, which
-// took a decode step of 64 x 8192 positions from 176 to TBD us.
+// cost a decode step of 61 x 1000 positions 27.4 us instead of 25.3.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
@@ -142,9 +142,9 @@ struct Span {
 __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int b) {
   Span s;
   s.len = a.lens ? min(max(a.lens[b], 0), a.seq_len) : a.seq_len;
-  const int64_t ctx = static_cast<int64_t>(max(a.ctx_lens[b], 0)) + a.ctx_add;
-  s.pos = ctx - s.len;
-  s.cut = static_cast<int>(min(ctx, static_cast<int64_t>(a.max_ctx)));
+  const int ctx = max(a.ctx_lens[b], 0);
+  s.pos = static_cast<int64_t>(ctx) - s.len;
+  s.cut = min(ctx, a.max_ctx);
   return s;
 }
 
@@ -159,11 +159,18 @@ __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n
 
 // Four values from element i on (a multiple of 4) of the output.
 __device__ __forceinline__ void store4(const PagedAttnArgs& a, int64_t i, f32x4_t v) {
-  if (a.out_dtype == DT_F32)
+  if (a.dtype == DT_F32)
     *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + i) = v;
   else
     *reinterpret_cast<u32x2_t*>(static_cast<bf16_t*>(a.out) + i) =
         u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+
+// Four values from element i on of a tensor in dtype.
+__device__ __forceinline__ f32x4_t load4(const void* p, int dtype, int64_t i) {
+  if (dtype == DT_F32) return *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + i);
+  const u32x2_t w = *reinterpret_cast<const u32x2_t*>(static_cast<const bf16_t*>(p) + i);
+  return f32x4_t{bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
 }
 
 // Over lanes l and l ^ 32.
@@ -195,7 +202,7 @@ struct Div {
 // How a call is cut (plan_of): splits of split_len positions; few rows: the
 // waves that share a row tile, a power of two.
 struct Plan {
-  bool big, aligned;  // aligned: four neighbouring positions share a page
+  bool big, aligned, join;  // aligned: four neighbouring positions share a page
   int n_split, split_len, waves_per_tile;
   int group, tile_groups;  // query heads per K/V head; blocks that a sequence's rows take in a split
   Div batch_div, split_div, kv_div, group_div, block_div, head_div, len_div;  // batch, n_split, n_head_kv, group, block_size, n_head, split_len
@@ -329,7 +336,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
       const int d = D >= 64 ? 16 * (q4 + 4 * (s / 2)) + 8 * (s % 2) : 8 * q4;
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (token < span.len && d < D) {
-        if (kTerms == 1) {
+        if (kTerms == 1 && !a.k_new) {
           const u32x4_t w = *reinterpret_cast<const u32x4_t*>(static_cast<const bf16_t*>(a.q) + at + d);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -604,7 +611,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
     stat[(kWaves + wave) * kRows + lane] = l;
   }
   __syncthreads();
-  if (len <= 0 && plan.n_split > 1) return;  // the join reads only the splits with positions
+  if (len <= 0 && plan.join) return;  // the join reads only the splits with positions
   const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
   for (int i = part_wave * kWave + lane; i < kRows * D / 4; i += wpt * kWave) {
     const int r = i / (D / 4), d = i % (D / 4) * 4, t = plan.group_div(row0 + r), h = kvh * G + row0 + r - t * G;
@@ -612,11 +619,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
     const int w0 = wave - part_wave;
     float M = stat[w0 * kRows + r];
     for (int w = 1; w < wpt; ++w) M = fmaxf(M, stat[(w0 + w) * kRows + r]);
-    const int zeros = plan.n_split == 1 && t < span.len ? max(a.zero_to - span.cut, 0) : 0;
-    if (zeros > 0) M = fmaxf(M, 0.f);
     const float base = finite_base(M) * c2;
     f32x4_t x{0.f, 0.f, 0.f, 0.f};
-    float L = zeros > 0 ? static_cast<float>(zeros) * __builtin_amdgcn_exp2f(-base) : 0.f;
+    float L = 0.f;
     for (int w = 0; w < wpt; ++w) {
       const float f = __builtin_amdgcn_exp2f(fmaf(stat[(w0 + w) * kRows + r], c2, -base));  // 0 without positions
       const f32x4_t y = *reinterpret_cast<const f32x4_t*>(lds + (w0 + w) * R::kWaveB + 16 * i);
@@ -625,7 +630,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
       L = fmaf(f, stat[(kWaves + w0 + w) * kRows + r], L);
     }
     const int64_t row = (static_cast<int64_t>(b) * a.seq_len + t) * a.n_head + h;
-    if (plan.n_split == 1) {
+    if (!plan.join) {
       const bool none = t >= span.len || L == 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : x[e] / L;
@@ -1062,14 +1067,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
   const int64_t row = (static_cast<int64_t>(b) * a.seq_len + token) * a.n_head + head;
   const int64_t n_rows = static_cast<int64_t>(a.batch) * a.seq_len * a.n_head;
   if (n_split == 1) {
-    const int zeros = token < span.len ? max(a.zero_to - span.cut, 0) : 0;
-    float f = 1.f;
-    if (zeros > 0) {
-      const float top = fmaxf(m, 0.f);
-      f = __builtin_amdgcn_exp2f((m - top) * c2);
-      l = fmaf(l, f, static_cast<float>(zeros) * __builtin_amdgcn_exp2f(-top * c2));
-    }
-    f = token >= span.len || l == 0.f ? 0.f : f / l;
+    const float f = token >= span.len || l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -1098,10 +1096,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 // the row, its groups of lanes every kGroups-th split, and the groups are
 // merged in order.  Bound by latency: the first splits' statistics and
 // outputs are asked for beside the lengths that say which of them count (the
-// others' memory is there, and not used).
+// others' memory is there, and not used).  A decode step's own token and its
+// positions of zeros (score 0, value 0) are one more split: its key and value
+// as they were projected, not yet rounded to codes, against q in fp32.
 constexpr int kJoin = 8;  // splits of a round
 
-template <int D, bool kWide>
+template <int D, bool kWide, bool kStep>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, Plan plan) {
   constexpr int kLanes = D / 4, kGroups = kWide ? kThreads / kLanes : 1;
   constexpr int kRound = kWide ? 4 : kJoin;
@@ -1128,10 +1128,23 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, P
   const int t = plan.head_div(i);
   const Span span = span_of(a, b);
   const int limit = limit_of(a, span, t), used = limit > 0 ? plan.len_div(limit - 1) + 1 : 0;
-  const int zeros = t < span.len && g == 0 ? max(a.zero_to - span.cut, 0) : 0;
   const float c2 = a.scale * kLog2e;
-  float M = zeros > 0 ? 0.f : -INFINITY, L = static_cast<float>(zeros);
+  float M = -INFINITY, L = 0.f;
   f32x4_t o{0.f, 0.f, 0.f, 0.f};
+  if (kStep && g == 0) {
+    const f32x4_t qv = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.q) + row * D + d);
+    const int64_t kv = (static_cast<int64_t>(b) * a.n_head_kv + plan.group_div(i)) * D + d;
+    const f32x4_t kn = load4(a.k_new, a.dtype, kv), vn = load4(a.v_new, a.dtype, kv);
+    float dot = fmaf(qv[3], kn[3], fmaf(qv[2], kn[2], fmaf(qv[1], kn[1], qv[0] * kn[0])));
+#pragma unroll
+    for (int w = kLanes / 2; w > 0; w /= 2) dot += __shfl_xor(dot, w, kLanes);
+    const int zeros = a.max_ctx - span.cut;
+    M = zeros > 0 ? fmaxf(dot, 0.f) : dot;
+    const float base = finite_base(M) * c2, f = __builtin_amdgcn_exp2f(fmaf(dot, c2, -base));
+    L = zeros > 0 ? fmaf(static_cast<float>(zeros), __builtin_amdgcn_exp2f(-base), f) : f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = f * vn[e];
+  }
   for (int s0 = g; s0 < used; s0 += kRound * kGroups) {
     if (s0 > g) load(s0);
     float top = M;
@@ -1190,14 +1203,16 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, P
 constexpr double kBigPairs = 12 << 20;
 constexpr int kBigFrom = 32;
 
-Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int block_size, int q_dtype) {
+Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim, int block_size, int dtype,
+             bool step) {
   const int64_t rows = static_cast<int64_t>(seq_len) * (n_head / n_head_kv);
   const int64_t pairs = static_cast<int64_t>(batch) * n_head_kv;
   Plan p;
   p.aligned = block_size % 4 == 0;
-  p.big = q_dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom && static_cast<double>(pairs) * rows * max_ctx >= kBigPairs;
+  p.big = !step && dtype == DT_BF16 && head_dim >= 64 && rows >= kBigFrom &&
+          static_cast<double>(pairs) * rows * max_ctx >= kBigPairs;
   int64_t blocks, n;
-  int step;
+  int quantum;
   if (p.big) {
     p.waves_per_tile = 1;
     blocks = pairs * ((rows + kBigRows - 1) / kBigRows);
@@ -1205,7 +1220,7 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
     // Two splits of causal prompts are not worth joining (1024 tokens of 1024:
     // 48 against 38 us with one).
     if (n == 2 && max_ctx < 4ll * seq_len) n = 1;
-    step = 2 * kBigTile;
+    quantum = 2 * kBigTile;
   } else {
     // About 1024 waves, one per SIMD, which keep the memory as busy as twice
     // as many (64 x 8192 positions 176 against 171 us) and spend half the
@@ -1222,14 +1237,15 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
       n /= 2;
     }
     blocks = batch * ((tiles * p.waves_per_tile + kWaves - 1) / kWaves);
-    step = kChunk * p.waves_per_tile;
+    quantum = kChunk * p.waves_per_tile;
   }
   if (n < 1) n = 1;
   int64_t len = (max_ctx + n - 1) / n;
-  len = (len + step - 1) / step * step;
-  if (len < step) len = step;
+  len = (len + quantum - 1) / quantum * quantum;
+  if (len < quantum) len = quantum;
   n = (max_ctx + len - 1) / len;
   p.n_split = static_cast<int>(n < 1 ? 1 : n);
+  p.join = step || p.n_split > 1;
   p.split_len = static_cast<int>(len);
   p.group = n_head / n_head_kv;
   p.tile_groups = static_cast<int>(blocks / batch);
@@ -1264,22 +1280,26 @@ hipError_t launch_attn(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
 
 template <int D>
 hipError_t launch_dim(const PagedAttnArgs& a, hipStream_t s) {
-  const Plan p = plan_of(a.batch, a.seq_len, a.max_ctx, a.n_head, a.n_head_kv, D, a.block_size, a.q_dtype);
+  const Plan p = plan_of(a.batch, a.seq_len, a.max_ctx, a.n_head, a.n_head_kv, D, a.block_size, a.dtype,
+                         a.k_new != nullptr);
   hipError_t e = hipErrorNotSupported;
   if (p.big) {
     if constexpr (D >= 64) e = launch_attn<paged_tile_kernel<D>, Big<D>::kLds>(a, p, s);
-  } else if (a.q_dtype == DT_F32) {
+  } else if (a.dtype == DT_F32) {
     e = launch_attn<paged_stream_kernel<D, 3>, Stream<D>::kLds>(a, p, s);
   } else {
     e = launch_attn<paged_stream_kernel<D, 1>, Stream<D>::kLds>(a, p, s);
   }
   if (e != hipSuccess) return e;
-  if (p.n_split > 1) {
+  if (p.join) {
     const int rows = a.seq_len * a.n_head, per_block = kThreads / (D / 4);
-    if (p.n_split > kJoin)
-      hipLaunchKernelGGL((paged_join_kernel<D, true>), dim3(rows, a.batch), dim3(kThreads), 0, s, a, p);
+    const bool wide = p.n_split > kJoin;
+    const dim3 grid(wide ? rows : (rows + per_block - 1) / per_block, a.batch);
+    if (a.k_new)
+      hipLaunchKernelGGL((wide ? paged_join_kernel<D, true, true> : paged_join_kernel<D, false, true>), grid,
+                         dim3(kThreads), 0, s, a, p);
     else
-      hipLaunchKernelGGL((paged_join_kernel<D, false>), dim3((rows + per_block - 1) / per_block, a.batch),
+      hipLaunchKernelGGL((wide ? paged_join_kernel<D, true, false> : paged_join_kernel<D, false, false>), grid,
                          dim3(kThreads), 0, s, a, p);
   }
   return hipGetLastError();
@@ -1292,10 +1312,10 @@ bool paged_attn_supported(int head_dim) {
 }
 
 size_t paged_attn_workspace_floats(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim,
-                                   int q_dtype) {
+                                   int dtype, bool step) {
   if (batch == 0 || seq_len == 0) return 0;
-  const Plan p = plan_of(batch, seq_len, max_ctx, n_head, n_head_kv, head_dim, 1, q_dtype);
-  if (p.n_split <= 1) return 0;
+  const Plan p = plan_of(batch, seq_len, max_ctx, n_head, n_head_kv, head_dim, 1, dtype, step);
+  if (!p.join) return 0;
   return static_cast<size_t>(batch) * seq_len * n_head * p.n_split * (head_dim + 2);
 }
 

@@ -773,7 +773,8 @@ struct AttnLayout {
   size_t order, offsets, tables, lens, qkv, q_rot, k_new, v_new, part, attn, y, total;
 };
 
-AttnLayout attn_layout(const AttnShape& a, int64_t max_ctx, int act) {
+// `codes`: the pools hold e4m3 codes (attention_paged.hip's splits).
+AttnLayout attn_layout(const AttnShape& a, int64_t max_ctx, int act, bool codes = false) {
   AttnLayout L;
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -790,7 +791,12 @@ AttnLayout attn_layout(const AttnShape& a, int64_t max_ctx, int act) {
   L.q_rot = take(static_cast<size_t>(a.B) * a.n_embd * 4);
   L.k_new = take(static_cast<size_t>(a.B) * a.n_embd_kv * ab);
   L.v_new = take(static_cast<size_t>(a.B) * a.n_embd_kv * ab);
-  L.part = take(static_cast<size_t>(a.B) * a.n_head * attn_decode_splits(static_cast<int>(max_ctx)) * (a.D + 2) * 4);
+  L.part = take((codes ? paged_attn_workspace_floats(static_cast<int>(a.B), 1, static_cast<int>(max_ctx),
+                                                     static_cast<int>(a.n_head), static_cast<int>(a.n_head_kv),
+                                                     static_cast<int>(a.D), act, true)
+                       : static_cast<size_t>(a.B) * a.n_head * attn_decode_splits(static_cast<int>(max_ctx)) *
+                             (a.D + 2)) *
+                4);
   L.attn = take(static_cast<size_t>(a.B) * a.n_embd * ab);
   L.y = take(static_cast<size_t>(a.B) * a.n_embd * 4 * kLinearMaxSplit);
   L.total = off;
@@ -919,12 +925,14 @@ struct AttnWeights {
 
 // Projections, RoPE, attention over the pools and the output projection
 // (attention_block_decode.mlir:96-233).  k_new / v_new: [B, n_embd_kv] in
-// act dtype (RoPE applied to k_new).
+// act dtype (RoPE applied to k_new).  k_scales / v_scales non-null: pools of
+// e4m3 codes, and k_new / v_new are appended to them behind the attention.
 int run_attention(const AttnShape& a, const AttnWeights& w, const void* input, const int64_t* positions,
                   const void* k_pool, const void* v_pool, int64_t n_blocks, int block_size, const int* tables,
                   int max_blocks, const int* lens, int max_ctx, int act, void* out, void* k_new, void* v_new,
                   void* workspace, const AttnLayout& L, hipStream_t s, const void* residual = nullptr,
-                  const KvScatterDecode* scatter = nullptr) {
+                  const KvScatterDecode* scatter = nullptr, float* k_scales = nullptr,
+                  float* v_scales = nullptr) {
   const int B = static_cast<int>(a.B);
   const int nq = static_cast<int>(a.n_embd), nkv = static_cast<int>(a.n_embd_kv);
   int* order = at<int>(workspace, L.order);
@@ -965,9 +973,56 @@ int run_attention(const AttnShape& a, const AttnWeights& w, const void* input, c
   const float scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(a.D)));
   {
     ScopedTimer t(FMOE_TIMER_ATTENTION, s);
-    FMOE_HIP(launch_attn_decode(q_rot, k_pool, v_pool, n_blocks, block_size, tables, max_blocks, lens, max_ctx, k_new,
-                                v_new, B, static_cast<int>(a.n_head), static_cast<int>(a.n_head_kv),
-                                static_cast<int>(a.D), act, scale, at<float>(workspace, L.part), attn, s, scatter));
+    if (k_scales) {
+      PagedAttnArgs p{};
+      p.q = q_rot;
+      p.q_stride = nq;
+      p.dtype = act;
+      p.k_pool = static_cast<const uint8_t*>(k_pool);
+      p.v_pool = static_cast<const uint8_t*>(v_pool);
+      p.k_scales = k_scales;
+      p.v_scales = v_scales;
+      p.tables = tables;
+      p.ctx_lens = lens;
+      p.n_blocks = n_blocks;
+      p.block_size = block_size;
+      p.max_blocks = max_blocks;
+      p.max_ctx = max_ctx;
+      p.batch = B;
+      p.seq_len = 1;
+      p.n_head = static_cast<int>(a.n_head);
+      p.n_head_kv = static_cast<int>(a.n_head_kv);
+      p.head_dim = static_cast<int>(a.D);
+      p.scale = scale;
+      p.k_new = k_new;
+      p.v_new = v_new;
+      p.out = attn;
+      p.part = at<float>(workspace, L.part);
+      FMOE_HIP(launch_paged_attn(p, s));
+      // a table of one page a sequence, in which the new token's position is its row
+      KvAppendArgs k{};
+      k.k_cache = scatter->k_cache;
+      k.v_cache = scatter->v_cache;
+      k.k_scales = k_scales;
+      k.v_scales = v_scales;
+      k.k = k_new;
+      k.v = v_new;
+      k.k_stride = k.v_stride = nkv;
+      k.tables = scatter->block_idx;
+      k.start = scatter->pos_idx;
+      k.n_blocks = n_blocks;
+      k.block_size = block_size;
+      k.max_blocks = 1;
+      k.batch = B;
+      k.seq_len = 1;
+      k.n_head_kv = static_cast<int>(a.n_head_kv);
+      while ((1 << k.log2_dim) < a.D) ++k.log2_dim;
+      FMOE_HIP(launch_kv_append(k, act, true, s));
+    } else {
+      FMOE_HIP(launch_attn_decode(q_rot, k_pool, v_pool, n_blocks, block_size, tables, max_blocks, lens, max_ctx,
+                                  k_new, v_new, B, static_cast<int>(a.n_head), static_cast<int>(a.n_head_kv),
+                                  static_cast<int>(a.D), act, scale, at<float>(workspace, L.part), attn, s, scatter));
+    }
   }
   float* y = at<float>(workspace, L.y);
   {
@@ -1521,8 +1576,9 @@ size_t fmoe_attention_decode_paged_workspace_bytes(int64_t batch, int64_t max_co
 }
 
 static int attention_paged(const void* input, const void* residual, const void* norm_w, float rms_eps,
-                           const int64_t* positions, void* k_cache, void* v_cache, int64_t n_blocks,
-                           int64_t block_size, int64_t layer, const int32_t* block_tables,
+                           const int64_t* positions, void* k_cache, void* v_cache, float* k_scales,
+                           float* v_scales, bool codes, int64_t n_blocks, int64_t block_size, int64_t layer,
+                           const int32_t* block_tables,
                            const int32_t* context_lens, int64_t n_layers, int64_t max_blocks_per_seq,
                            int64_t max_context_len, const int32_t* block_indices, const int32_t* pos_in_blocks,
                            const void* packed_wqkv, const float* wqkv_scales, const void* packed_wo,
@@ -1542,8 +1598,8 @@ int fmoe_attention_decode_paged(const void* input, const int64_t* positions, voi
                                 int64_t n_head_kv, int64_t n_embd, int64_t n_embd_kv, float rope_freq_base,
                                 float rope_freq_scale, int act_dtype, void* out, void* k_new, void* v_new,
                                 void* workspace, size_t workspace_bytes, void* stream) {
-  return attention_paged(input, nullptr, nullptr, 0.f, positions, k_cache, v_cache, n_blocks, block_size, layer,
-                         block_tables, context_lens, n_layers, max_blocks_per_seq, max_context_len, block_indices,
+  return attention_paged(input, nullptr, nullptr, 0.f, positions, k_cache, v_cache, nullptr, nullptr, false, n_blocks,
+                         block_size, layer, block_tables, context_lens, n_layers, max_blocks_per_seq, max_context_len, block_indices,
                          pos_in_blocks, packed_wqkv, wqkv_scales, packed_wo, wo_scales, w_dtype, bq, bk, bv, bo,
                          use_bias, batch, n_head, n_head_kv, n_embd, n_embd_kv, rope_freq_base, rope_freq_scale,
                          act_dtype, out, k_new, v_new, workspace, workspace_bytes, stream);
@@ -1572,8 +1628,8 @@ int fmoe_attention_sublayer_decode_paged(const void* residual, const void* attn_
                                          void* workspace, size_t workspace_bytes, void* stream) {
   if (batch > 0 && (!residual || !attn_norm_w)) return fail(FMOE_ERR_INVALID_ARGUMENT, "null pointer");
   if (batch > 0 && !aligned_for(attn_norm_w, act_dtype)) return fail(FMOE_ERR_INVALID_ARGUMENT, "misaligned pointer");
-  return attention_paged(residual, residual, attn_norm_w, rms_eps, positions, k_cache, v_cache, n_blocks, block_size,
-                         layer, block_tables, context_lens, n_layers, max_blocks_per_seq, max_context_len,
+  return attention_paged(residual, residual, attn_norm_w, rms_eps, positions, k_cache, v_cache, nullptr, nullptr,
+                         false, n_blocks, block_size, layer, block_tables, context_lens, n_layers, max_blocks_per_seq, max_context_len,
                          block_indices, pos_in_blocks, packed_wqkv, wqkv_scales, packed_wo, wo_scales, w_dtype, bq,
                          bk, bv, bo, use_bias, batch, n_head, n_head_kv, n_embd, n_embd_kv, rope_freq_base,
                          rope_freq_scale, act_dtype, out, k_new, v_new, workspace, workspace_bytes, stream);
@@ -1680,7 +1736,7 @@ size_t fmoe_attention_paged_workspace_bytes(int64_t batch, int64_t seq_len, int6
     return 0;
   return align_up(paged_attn_workspace_floats(static_cast<int>(batch), static_cast<int>(seq_len),
                                               static_cast<int>(max_context_len), static_cast<int>(n_head),
-                                              static_cast<int>(n_head_kv), static_cast<int>(head_dim), act_dtype) *
+                                              static_cast<int>(n_head_kv), static_cast<int>(head_dim), act_dtype, false) *
                   sizeof(float));
 }
 
@@ -1716,8 +1772,7 @@ int fmoe_attention_paged(const void* q, int64_t q_stride, const void* k_cache, c
   PagedAttnArgs a{};
   a.q = q;
   a.q_stride = q_stride;
-  a.q_dtype = act_dtype;
-  a.out_dtype = act_dtype;
+  a.dtype = act_dtype;
   a.k_pool = static_cast<const uint8_t*>(k_cache);
   a.v_pool = static_cast<const uint8_t*>(v_cache);
   a.k_scales = k_scales;
@@ -1742,6 +1797,69 @@ int fmoe_attention_paged(const void* q, int64_t q_stride, const void* k_cache, c
   return ok();
 }
 
+// The decode step over pools of e4m3 codes.
+size_t fmoe_attention_decode_paged_f8_workspace_bytes(int64_t batch, int64_t max_context_len, int64_t n_head,
+                                                      int64_t n_head_kv, int64_t n_embd, int64_t n_embd_kv,
+                                                      int act_dtype) {
+  if (!act_dtype_ok(act_dtype) || batch < 0 || batch > 65535 || max_context_len < 0 ||
+      max_context_len > kMaxPagedContext || n_head < 1 || n_head > 65535 || n_head_kv < 1 || n_head % n_head_kv ||
+      n_embd < n_head || n_embd > kMaxDim || n_embd_kv < 0 || n_embd_kv > kMaxDim)
+    return 0;
+  const AttnShape a{batch, n_head, n_head_kv, n_embd, n_embd_kv, n_embd / n_head};
+  return attn_layout(a, max_context_len, act_dtype, true).total;
+}
+
+int fmoe_attention_decode_paged_f8(const void* input, const int64_t* positions, void* k_cache, void* v_cache,
+                                   float* k_scales, float* v_scales, int64_t n_blocks, int64_t block_size,
+                                   int64_t layer, const int32_t* block_tables, const int32_t* context_lens,
+                                   int64_t n_layers, int64_t max_blocks_per_seq, int64_t max_context_len,
+                                   const int32_t* block_indices, const int32_t* pos_in_blocks,
+                                   const void* packed_wqkv, const float* wqkv_scales, const void* packed_wo,
+                                   const float* wo_scales, int w_dtype, const float* bq, const float* bk,
+                                   const float* bv, const float* bo, int use_bias, int64_t batch, int64_t n_head,
+                                   int64_t n_head_kv, int64_t n_embd, int64_t n_embd_kv, float rope_freq_base,
+                                   float rope_freq_scale, int act_dtype, void* out, void* k_new, void* v_new,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_paged(input, nullptr, nullptr, 0.f, positions, k_cache, v_cache, k_scales, v_scales, true, n_blocks,
+                         block_size, layer, block_tables, context_lens, n_layers, max_blocks_per_seq,
+                         max_context_len, block_indices, pos_in_blocks, packed_wqkv, wqkv_scales, packed_wo,
+                         wo_scales, w_dtype, bq, bk, bv, bo, use_bias, batch, n_head, n_head_kv, n_embd, n_embd_kv,
+                         rope_freq_base, rope_freq_scale, act_dtype, out, k_new, v_new, workspace, workspace_bytes,
+                         stream);
+}
+
+size_t fmoe_attention_sublayer_decode_paged_f8_workspace_bytes(int64_t batch, int64_t max_context_len, int64_t n_head,
+                                                               int64_t n_head_kv, int64_t n_embd, int64_t n_embd_kv,
+                                                               int act_dtype) {
+  const size_t base = fmoe_attention_decode_paged_f8_workspace_bytes(batch, max_context_len, n_head, n_head_kv, n_embd,
+                                                                     n_embd_kv, act_dtype);
+  if (base == 0) return 0;
+  return base + align_up(static_cast<size_t>(batch) * n_embd * dtype_bytes(act_dtype));
+}
+
+int fmoe_attention_sublayer_decode_paged_f8(const void* residual, const void* attn_norm_w, float rms_eps,
+                                            const int64_t* positions, void* k_cache, void* v_cache, float* k_scales,
+                                            float* v_scales, int64_t n_blocks, int64_t block_size, int64_t layer,
+                                            const int32_t* block_tables, const int32_t* context_lens,
+                                            int64_t n_layers, int64_t max_blocks_per_seq, int64_t max_context_len,
+                                            const int32_t* block_indices, const int32_t* pos_in_blocks,
+                                            const void* packed_wqkv, const float* wqkv_scales, const void* packed_wo,
+                                            const float* wo_scales, int w_dtype, const float* bq, const float* bk,
+                                            const float* bv, const float* bo, int use_bias, int64_t batch,
+                                            int64_t n_head, int64_t n_head_kv, int64_t n_embd, int64_t n_embd_kv,
+                                            float rope_freq_base, float rope_freq_scale, int act_dtype, void* out,
+                                            void* k_new, void* v_new, void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+  if (batch > 0 && (!residual || !attn_norm_w)) return fail(FMOE_ERR_INVALID_ARGUMENT, "null pointer");
+  if (batch > 0 && !aligned_for(attn_norm_w, act_dtype)) return fail(FMOE_ERR_INVALID_ARGUMENT, "misaligned pointer");
+  return attention_paged(residual, residual, attn_norm_w, rms_eps, positions, k_cache, v_cache, k_scales, v_scales,
+                         true, n_blocks, block_size, layer, block_tables, context_lens, n_layers, max_blocks_per_seq,
+                         max_context_len, block_indices, pos_in_blocks, packed_wqkv, wqkv_scales, packed_wo,
+                         wo_scales, w_dtype, bq, bk, bv, bo, use_bias, batch, n_head, n_head_kv, n_embd, n_embd_kv,
+                         rope_freq_base, rope_freq_scale, act_dtype, out, k_new, v_new, workspace, workspace_bytes,
+                         stream);
+}
+
 }  // extern "C"
 
 // Shared by the paged attention and the attention sub-layer: norm_w non-null
@@ -1749,8 +1867,9 @@ int fmoe_attention_paged(const void* q, int64_t q_stride, const void* k_cache, c
 // transformer_layer_moe_decode.mlir:174-177) and `residual` is added to the
 // output (:208-221).
 static int attention_paged(const void* input, const void* residual, const void* norm_w, float rms_eps,
-                           const int64_t* positions, void* k_cache, void* v_cache, int64_t n_blocks,
-                           int64_t block_size, int64_t layer, const int32_t* block_tables,
+                           const int64_t* positions, void* k_cache, void* v_cache, float* k_scales,
+                           float* v_scales, bool codes, int64_t n_blocks, int64_t block_size, int64_t layer,
+                           const int32_t* block_tables,
                            const int32_t* context_lens, int64_t n_layers, int64_t max_blocks_per_seq,
                            int64_t max_context_len, const int32_t* block_indices, const int32_t* pos_in_blocks,
                            const void* packed_wqkv, const float* wqkv_scales, const void* packed_wo,
@@ -1766,7 +1885,7 @@ static int attention_paged(const void* input, const void* residual, const void* 
   FMOE_TRY(check_dims("n_layers", n_layers, 1, kMaxDim));
   FMOE_TRY(check_dims("layer", layer, 0, n_layers - 1));
   FMOE_TRY(check_dims("max_blocks_per_seq", max_blocks_per_seq, 1, kMaxDim));
-  FMOE_TRY(check_dims("max_context_len", max_context_len, 0, kMaxDim));
+  FMOE_TRY(check_dims("max_context_len", max_context_len, 0, codes ? kMaxPagedContext : kMaxDim));
   const AttnWeights w{packed_wqkv, wqkv_scales, packed_wo, wo_scales, w_dtype, bq, bk, bv, bo, use_bias,
                       rope_freq_base, rope_freq_scale};
   FMOE_TRY(check_attn_weights(w));
@@ -1774,12 +1893,15 @@ static int attention_paged(const void* input, const void* residual, const void* 
   if (!input || !positions || !k_cache || !v_cache || !block_tables || !context_lens || !block_indices ||
       !pos_in_blocks || !out || !workspace)
     return fail(FMOE_ERR_INVALID_ARGUMENT, "null pointer");
+  if (codes && (!k_scales || !v_scales)) return fail(FMOE_ERR_INVALID_ARGUMENT, "a cache of codes needs scales");
   if (reinterpret_cast<uintptr_t>(k_cache) % 16 || reinterpret_cast<uintptr_t>(v_cache) % 16)
     return fail(FMOE_ERR_INVALID_ARGUMENT, "K/V pools must be 16-byte aligned");
+  if (codes && ((k_new && !aligned16(k_new)) || (v_new && !aligned16(v_new))))
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "k_new and v_new must be 16-byte aligned");
   if (!aligned_for(input, act_dtype) || !aligned_for(out, act_dtype) || (k_new && !aligned_for(k_new, act_dtype)) ||
       (v_new && !aligned_for(v_new, act_dtype)))
     return fail(FMOE_ERR_INVALID_ARGUMENT, "misaligned pointer");
-  const AttnLayout L = attn_layout(a, max_context_len, act_dtype);
+  const AttnLayout L = attn_layout(a, max_context_len, act_dtype, codes);
   const size_t xn_off = L.total;
   const size_t need = norm_w ? xn_off + align_up(static_cast<size_t>(batch) * n_embd * dtype_bytes(act_dtype))
                              : L.total;
@@ -1808,6 +1930,6 @@ static int attention_paged(const void* input, const void* residual, const void* 
   FMOE_TRY(run_attention(a, w, x, positions, k_cache, v_cache, n_blocks, static_cast<int>(block_size),
                          block_tables + layer * batch * max_blocks_per_seq, static_cast<int>(max_blocks_per_seq),
                          context_lens + layer * batch, static_cast<int>(max_context_len), act_dtype, out, kn, vn,
-                         workspace, L, s, residual, &sc));
+                         workspace, L, s, residual, &sc, k_scales, v_scales));
   return ok();
 }

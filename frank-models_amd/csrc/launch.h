@@ -434,14 +434,15 @@ hipError_t launch_kv_append(const KvAppendArgs& args, int act, bool codes, hipSt
 
 // ---- attention over e4m3 pages (attention_paged.hip)
 // Query (b, s, h) at ((b * seq_len + s) * q_stride + h * head_dim), one of the
-// last lens[b] (null: seq_len) tokens of a context of ctx_lens[b] + ctx_add,
-// against positions below min(context, max_ctx) and, causal, up to its own.
-// zero_to: positions from the context's end to it are keys and values of
-// zeros that every query attends (0: none).
+// last lens[b] (null: seq_len) tokens of a context of ctx_lens[b], against
+// positions below min(context, max_ctx) and, causal, up to its own.
+// k_new non-null: a decode step (seq_len 1, causal 0, q in fp32), whose query
+// also attends k_new / v_new [batch, n_head_kv, head_dim] (in dtype) and
+// positions from the context's end to max_ctx as keys and values of zeros.
 struct PagedAttnArgs {
   const void* q;
   int64_t q_stride;
-  int q_dtype, out_dtype;
+  int dtype;  // of out and, but for a decode step, q
   const uint8_t* k_pool;  // [n_blocks, block_size, n_head_kv, head_dim]
   const uint8_t* v_pool;
   const float* k_scales;  // [n_blocks, n_head_kv]
@@ -451,14 +452,16 @@ struct PagedAttnArgs {
   const int* lens;      // [batch] or null
   int64_t n_blocks;
   int block_size, max_blocks, max_ctx, batch, seq_len, n_head, n_head_kv, head_dim;
-  int ctx_add, zero_to, causal;
+  int causal;
   float scale;
+  const void* k_new;
+  const void* v_new;
   void* out;    // [batch, seq_len, n_head, head_dim]
   float* part;  // paged_attn_workspace_floats
 };
 bool paged_attn_supported(int head_dim);
 size_t paged_attn_workspace_floats(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int head_dim,
-                                   int q_dtype);
+                                   int dtype, bool step);
 hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s);
 
 }  // namespace fmoe

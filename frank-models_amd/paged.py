@@ -15,86 +15,21 @@ comes back as NumPy.  Pools are device tensors, updated in place.
 from __future__ import annotations
 
 import functools
-from dataclasses import dataclass
 
 import torch
 
 from . import _lib as L
 from .api import _TORCH_TO_DT, _device, _finish, _to_device
 from .attention import _ints_to_device
+from .kvpool import QuantizedKVPool, check_pools, here
 
 # A decode step makes a call of each per layer, whose kernels take a few
 # microseconds: the checks ask tensors for plain numbers (device index, shape,
 # strides) and leave what is in order as it is.
 
 
-def _here() -> int:
-    """The current device's index."""
-    if not torch.cuda.is_initialized():
-        _device()  # NoDeviceError where there is none
-    return torch.cuda.current_device()
-
-
 def _raw_stream(dev: int) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
-
-
-@dataclass
-class QuantizedKVPool:
-    """A K or V pool in OCP fp8-e4m3: ``data [n_blocks, block_size, n_head_kv,
-    head_dim]`` (torch.float8_e4m3fn or uint8 codes) and ``scales [n_blocks,
-    n_head_kv]`` float32, both contiguous on the device.  A value is
-    ``decode(data) * scales`` of its block and head."""
-
-    data: torch.Tensor
-    scales: torch.Tensor
-
-    @classmethod
-    def zeros(cls, n_blocks: int, block_size: int, n_head_kv: int, head_dim: int) -> "QuantizedKVPool":
-        dev = _device()
-        data = torch.zeros((n_blocks, block_size, n_head_kv, head_dim), dtype=torch.uint8, device=dev)
-        return cls(data.view(torch.float8_e4m3fn), torch.zeros((n_blocks, n_head_kv), dtype=torch.float32, device=dev))
-
-    @property
-    def shape(self):
-        return tuple(self.data.shape)
-
-    def dequantize(self) -> torch.Tensor:
-        """The values, float32."""
-        return self.data.view(torch.float8_e4m3fn).float() * self.scales[:, None, :, None]
-
-
-_CODES = (torch.float8_e4m3fn, torch.uint8)
-
-
-def _check_pool(pool, name, dev):
-    """-> (data, scales or None, shape) of a pool argument, checked."""
-    quantized = isinstance(pool, QuantizedKVPool)
-    data, scales = (pool.data, pool.scales) if quantized else (pool, None)
-    if not isinstance(data, torch.Tensor) or data.get_device() != dev or not data.is_contiguous():
-        raise TypeError(f"{name} must be a contiguous tensor on the current device, cuda:{dev}")
-    shape = data.shape
-    if len(shape) != 4:
-        raise ValueError(f"{name} must be [n_blocks, block_size, n_head_kv, head_dim], got {tuple(shape)}")
-    if quantized:
-        if data.dtype not in _CODES:
-            raise TypeError(f"{name}: codes must be float8_e4m3fn or uint8, got {data.dtype}")
-        if (not isinstance(scales, torch.Tensor) or scales.dtype is not torch.float32 or scales.get_device() != dev
-                or not scales.is_contiguous()):
-            raise TypeError(f"{name}: scales must be a contiguous float32 tensor on the current device, cuda:{dev}")
-        if scales.shape != (shape[0], shape[2]):
-            raise ValueError(f"{name}: scales must be [n_blocks, n_head_kv] = [{shape[0]}, {shape[2]}]")
-    return data, scales, shape
-
-
-def _check_pools(k_cache, v_cache, dev):
-    k, ks, shape = _check_pool(k_cache, "k_cache", dev)
-    v, vs, v_shape = _check_pool(v_cache, "v_cache", dev)
-    if shape != v_shape or (ks is None) != (vs is None) or (ks is None and k.dtype is not v.dtype):
-        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v_shape)} must have one shape and type")
-    if k.data_ptr() == v.data_ptr() and k.numel():
-        raise ValueError("k_cache and v_cache must be two pools")
-    return k, ks, v, vs, shape
 
 
 def _tokens(x, name, heads, dim, dev):
@@ -173,8 +108,8 @@ def kvcache_append(k_cache, v_cache, layer: int, k, v, block_tables, start_posit
     nothing.  Positions without a block in the pool are skipped; a block
     that the call's tables name several times is written by the last
     sequence and position alone."""
-    dev = _here()
-    kc, ks, vc, vs, (n_blocks, bs, hkv, d) = _check_pools(k_cache, v_cache, dev)
+    dev = here()
+    kc, ks, vc, vs, (n_blocks, bs, hkv, d) = check_pools(k_cache, v_cache, dev)
     k, k_stride, shape, _ = _tokens(k, "k", hkv, d, dev)
     v, v_stride, v_shape, _ = _tokens(v, "v", hkv, d, dev)
     dtype = k.dtype
@@ -229,10 +164,10 @@ def attention_paged(q, k_cache, v_cache, layer: int, block_tables, context_lens,
     up to its own; ``scale`` defaults to ``1 / sqrt(head_dim)``.  Tokens that
     attend nothing, and padding tokens, get zeros.  ``out`` must not overlap
     ``q``."""
-    dev = _here()
+    dev = here()
     if not isinstance(k_cache, QuantizedKVPool) or not isinstance(v_cache, QuantizedKVPool):
         raise TypeError("attention_paged reads QuantizedKVPool caches")
-    kc, ks, vc, vs, (n_blocks, bs, hkv, d) = _check_pools(k_cache, v_cache, dev)
+    kc, ks, vc, vs, (n_blocks, bs, hkv, d) = check_pools(k_cache, v_cache, dev)
     q, q_stride, shape, from_np = _tokens(q, "q", None, d, dev)
     batch, seq_len, n_head, _ = shape
     dtype = q.dtype

@@ -485,6 +485,49 @@ int fmoe_attention_paged(const void *q, int64_t q_stride, const void *k_cache,
                          float scale, int act_dtype, void *out, void *workspace,
                          size_t workspace_bytes, void *stream);
 
+/* fmoe_attention_decode_paged and fmoe_attention_sublayer_decode_paged over
+ * pools of e4m3 codes.  The query attends the codes, rounded to act_dtype for
+ * it, and its own key and value in act_dtype; the append of the new K/V to
+ * slot (block_indices, pos_in_blocks) follows fmoe_kvcache_append: the page's
+ * rows below pos_in_blocks are taken to be in use, and of sequences that name
+ * one page the last alone writes it.  k_new / v_new: 16-byte aligned or null.
+ * max_context_len at most 2^31 - 4097. */
+size_t fmoe_attention_decode_paged_f8_workspace_bytes(int64_t batch, int64_t max_context_len,
+                                                      int64_t n_head, int64_t n_head_kv,
+                                                      int64_t n_embd, int64_t n_embd_kv,
+                                                      int act_dtype);
+int fmoe_attention_decode_paged_f8(const void *input, const int64_t *positions, void *k_cache,
+                                   void *v_cache, float *k_scales, float *v_scales,
+                                   int64_t n_blocks, int64_t block_size, int64_t layer,
+                                   const int32_t *block_tables, const int32_t *context_lens,
+                                   int64_t n_layers, int64_t max_blocks_per_seq,
+                                   int64_t max_context_len, const int32_t *block_indices,
+                                   const int32_t *pos_in_blocks, const void *packed_wqkv,
+                                   const float *wqkv_scales, const void *packed_wo,
+                                   const float *wo_scales, int w_dtype, const float *bq,
+                                   const float *bk, const float *bv, const float *bo,
+                                   int use_bias, int64_t batch, int64_t n_head, int64_t n_head_kv,
+                                   int64_t n_embd, int64_t n_embd_kv, float rope_freq_base,
+                                   float rope_freq_scale, int act_dtype, void *out, void *k_new,
+                                   void *v_new, void *workspace, size_t workspace_bytes,
+                                   void *stream);
+size_t fmoe_attention_sublayer_decode_paged_f8_workspace_bytes(int64_t batch,
+                                                               int64_t max_context_len,
+                                                               int64_t n_head, int64_t n_head_kv,
+                                                               int64_t n_embd, int64_t n_embd_kv,
+                                                               int act_dtype);
+int fmoe_attention_sublayer_decode_paged_f8(
+    const void *residual, const void *attn_norm_w, float rms_eps, const int64_t *positions,
+    void *k_cache, void *v_cache, float *k_scales, float *v_scales, int64_t n_blocks,
+    int64_t block_size, int64_t layer, const int32_t *block_tables, const int32_t *context_lens,
+    int64_t n_layers, int64_t max_blocks_per_seq, int64_t max_context_len,
+    const int32_t *block_indices, const int32_t *pos_in_blocks, const void *packed_wqkv,
+    const float *wqkv_scales, const void *packed_wo, const float *wo_scales, int w_dtype,
+    const float *bq, const float *bk, const float *bv, const float *bo, int use_bias, int64_t batch,
+    int64_t n_head, int64_t n_head_kv, int64_t n_embd, int64_t n_embd_kv, float rope_freq_base,
+    float rope_freq_scale, int act_dtype, void *out, void *k_new, void *v_new, void *workspace,
+    size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,8 @@ import numpy as np
 import pytest
 import torch
 
+from helpers import assert_close_rms
+from oracle import attention as oa
 from oracle import numerics as nm
 from oracle import paged as op
 
@@ -467,6 +469,142 @@ def test_prompt_then_decode(fm, act):
                 v = values[1][table[b, j // bs], j % bs]
                 scale = vp.scales.cpu().numpy()[table[b, j // bs]][:, None]
                 assert np.all(np.abs(v - x[2][b, i]) <= 2.0 ** -4 * np.abs(x[2][b, i]) + 2.0 ** -10 * scale)
+
+
+# ---------------------------------------------------------------- the decode step
+def block(fm, rng, act, H, Hkv, D):
+    n, nkv = H * D, Hkv * D
+    w = [rounded(rng.standard_normal(s) / np.sqrt(n), act) for s in ((n, n), (n, nkv), (n, nkv), (n, n))]
+    b = [(rng.standard_normal(m) * 0.1).astype(np.float32) for m in (n, nkv, nkv, n)]
+    blk = fm.AttentionBlockDecode(*(dev(x, act) for x in w), *(dev(x) for x in b), use_bias=True, n_head=H,
+                                  n_head_kv=Hkv, n_embd=n, act_dtype=DT[act])
+    return blk, [*w, *b, True, H, Hkv, n]
+
+
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+@pytest.mark.parametrize("H,Hkv,D,bs,context,max_ctx", [
+    (4, 2, 16, 4, [10, 3, 0], 12),
+    (8, 1, 32, 16, [1, 64, 65], 65),
+    (4, 4, 64, 32, [700, 31, 2, 300], 500),  # cut, and positions of zeros
+    (8, 2, 128, 16, [5000, 4999, 17], 5000),  # a dozen splits and more
+    (16, 8, 64, 16, [40] * 130, 40),  # one split
+    (4, 2, 128, 16, [0, 0], 0),
+])
+def test_decode_step(fm, act, H, Hkv, D, bs, context, max_ctx):
+    """The decode step over codes: against the 64-bit one over the codes'
+    values, at the tolerances of the step over plain pools (which leave room
+    for the bf16 query and weights: 2^-8 of a score and of a weight, averaged
+    over the positions); what it appends bit for bit as the append does."""
+    rng = np.random.default_rng(H * D + len(context))
+    B, per = len(context), -(-(max(context) + 1) // bs)
+    n_blocks = B * per
+    table = rng.permutation(n_blocks).reshape(B, per)
+    slot = table[np.arange(B), np.asarray(context) // bs].copy()
+    table[0, (context[0] + 1) // bs // 2] = -5  # rows of zeros
+    if B > 3:
+        slot[1] = n_blocks  # nowhere
+    row = np.asarray(context) % bs
+    (kc, ks), (vc, vs) = (random_pool(rng, n_blocks, bs, Hkv, D) for _ in range(2))
+    blk, args = block(fm, rng, act, H, Hkv, D)
+    x, nw = rounded(rng.standard_normal((B, H * D)), act), rounded(rng.uniform(0.5, 1.5, H * D), act)
+    pos = np.asarray(context, np.int64)
+    tables, lens = (np.stack([np.full_like(t, 9 * n_blocks), t]).astype(np.int32) for t in (table, np.asarray(context)))
+    kf, vf = op.values(kc, ks), op.values(vc, vs)
+    good = np.where((tables >= 0) & (tables < n_blocks), tables, n_blocks)
+    paging = (1, good, lens, max_ctx, np.full(B, n_blocks), row)
+    rtol = 1e-4 if act == "f32" else 2e-2
+    for sublayer in (False, True):
+        kp, vp = gpu_pool(fm, kc, ks), gpu_pool(fm, vc, vs)
+        call = (kp, vp, 1, dev(tables), dev(lens), max_ctx, dev(slot.astype(np.int32)), dev(row.astype(np.int32)))
+        if sublayer:
+            out, k_new, v_new = blk.paged_sublayer(dev(x, act), dev(nw, act), 1e-5, dev(pos), *call)
+            ref = oa.attention_sublayer_decode_paged(x, nw, 1e-5, pos, kf, vf, *paging, *args)
+        else:
+            out, k_new, v_new = blk.paged(dev(x, act), dev(pos), *call)
+            ref = oa.attention_decode_paged(x, pos, kf, vf, *paging, *args)
+        for got, want in zip((out, k_new, v_new), ref):
+            assert_close_rms(got.float().cpu().numpy(), want, rtol)
+        codes = [a.copy() for a in (kc, ks, vc, vs)]
+        for (c, s), new in ((codes[:2], k_new), (codes[2:], v_new)):
+            op.append(c, s, new[:, None].double().cpu().numpy(), slot[:, None], row, np.ones(B))
+        for got, want in zip((codes_of(kp), kp.scales.cpu().numpy(), codes_of(vp), vp.scales.cpu().numpy()), codes):
+            assert np.array_equal(got, want)
+
+
+def test_decode_step_is_append_and_attention_of_codes(fm):
+    """Where the new token's key and value are codes exactly, the step over a
+    full context attends what append and attention do: weights of zero but for
+    the query's and small integers for the values."""
+    H, Hkv, D, bs, ctx = 2, 1, 64, 16, 37
+    n = H * D
+    zero, eye = torch.zeros(n, n, device="cuda"), torch.eye(n, device="cuda")
+    blk = fm.AttentionBlockDecode(zero, zero[:, :D].contiguous(), eye[:, :D].contiguous(), eye, n_head=H, n_head_kv=Hkv, n_embd=n,
+                                  act_dtype=torch.float32)
+    pools = [[fm.QuantizedKVPool.zeros(4, bs, Hkv, D) for _ in range(2)] for _ in range(2)]
+    table = dev(np.array([[[2, 0, 3]]], np.int32))
+    x = torch.randint(-8, 9, (ctx + 1, n), device="cuda").float()
+    kv = torch.zeros(1, ctx, Hkv, D, device="cuda"), x[:ctx, :D].reshape(1, ctx, Hkv, D).contiguous()
+    for p in pools:
+        fm.kvcache_append(*p, 0, *kv, table, dev(np.zeros(1, np.int32)))
+    out, k_new, v_new = blk.paged(x[ctx:], dev(np.array([ctx])), *pools[0], 0, table, dev(np.array([[ctx]], np.int32)), ctx,
+                                  dev(np.array([3], np.int32)), dev(np.array([5], np.int32)))
+    q = fm.kvcache_append(*pools[1], 0, k_new[:, None], v_new[:, None], table, dev(np.array([ctx], np.int32)),
+                          q=torch.zeros(1, 1, H, D, device="cuda"), rope=False)
+    ref = fm.attention_paged(q, *pools[1], 0, table, dev(np.array([[ctx + 1]], np.int32)), ctx + 1)
+    assert all(torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.scales, b.scales)
+               for a, b in zip(*pools))
+    # all scores are 0: the mean of integers, two roundings and a product each
+    mean = x[:, :D].double().mean(0).repeat(H)
+    for got in (out, ref.reshape(1, n)):
+        assert (got.double() - mean).abs().max() <= 8 * 2.0 ** -22
+
+
+def test_decode_step_captured(fm):
+    rng = np.random.default_rng(31)
+    B, H, Hkv, D, bs, ctx = 3, 8, 2, 128, 16, 900
+    blk, _ = block(fm, rng, "bf16", H, Hkv, D)
+    per = ctx // bs + 1
+    table = dev(rng.permutation(B * per).reshape(1, B, per).astype(np.int32))
+    cl = dev(np.array([[ctx, 500, 16]], np.int32))
+    slot = table[0].gather(1, (cl[0] // bs).long()[:, None])[:, 0].contiguous()
+    start = [random_pool(rng, B * per, bs, Hkv, D) for _ in range(2)]
+    x = torch.randn(B, H * D, device="cuda").bfloat16()
+    pools = [gpu_pool(fm, *s) for s in start]
+    call = lambda p, x: blk.paged(x, cl[0].long(), *p, 0, table, cl, ctx, slot, cl[0] % bs)[0]  # noqa: E731
+    call(pools, x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call(pools, x)
+    for _ in range(3):
+        x.copy_(torch.randn_like(x))
+        mine = [gpu_pool(fm, *s) for s in start]
+        for p, m in zip(pools, mine):
+            p.data.copy_(m.data)
+            p.scales.copy_(m.scales)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call(mine, x))
+        assert all(torch.equal(p.data.view(torch.uint8), m.data.view(torch.uint8)) and torch.equal(p.scales, m.scales)
+                   for p, m in zip(pools, mine))
+
+
+def test_decode_step_arguments(fm):
+    blk, _ = block(fm, np.random.default_rng(0), "f32", 4, 2, 16)
+    kp, vp = (fm.QuantizedKVPool.zeros(4, 4, 2, 16) for _ in range(2))
+    x, pos, bt = torch.zeros(1, 64, device="cuda"), dev(np.zeros(1, np.int64)), dev(np.zeros((1, 1, 1), np.int32))
+    one = dev(np.zeros(1, np.int32))
+    for exc, k, v in [(ValueError, kp, vp.dequantize()), (ValueError, kp.dequantize(), vp), (ValueError, kp, kp),
+                      (ValueError, *(fm.QuantizedKVPool.zeros(4, 4, 1, 16) for _ in range(2))),
+                      (TypeError, fm.QuantizedKVPool(kp.data.float(), kp.scales), vp),
+                      (ValueError, fm.QuantizedKVPool(kp.data, kp.scales[:2]), vp)]:
+        with pytest.raises(exc):
+            blk.paged(x, pos, k, v, 0, bt, bt[0], 4, one, one)
+    with pytest.raises(ValueError):
+        blk.paged(x, pos, kp, vp, 0, bt, bt[0], 2 ** 31 - 4096, one, one)
+    out, k_new, _ = blk.paged(x[:0], pos[:0], kp, vp, 0, bt[:, :0], bt[0, :0].view(1, 0), 4, one[:0], one[:0])
+    assert out.shape == (0, 64) and k_new.shape == (0, 2, 16)
 
 
 def test_captured_and_replayed(fm):
