@@ -183,22 +183,6 @@ __device__ __forceinline__ float sum_halves(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Division of 0 <= x < 2^31 by d: x m / 2^(31 + l) with m = 2^(31 + l) / d
-// rounded up and 2^l >= d, exact because x (m d - 2^(31 + l)) < 2^31 2^l.  The
-// hardware has no integer division; a call's kernels make a dozen before
-// their first load.
-struct Div {
-  uint32_t m, s;
-  static Div by(uint32_t d) {
-    uint32_t l = 0;
-    while ((1ull << l) < d) ++l;
-    return Div{static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d), 31 + l};
-  }
-  __device__ __forceinline__ int operator()(int x) const {
-    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * m >> s);
-  }
-};
-
 // How a call is cut (plan_of): splits of split_len positions; few rows: the
 // waves that share a row tile, a power of two.
 struct Plan {

@@ -291,4 +291,19 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int n
   return false;
 }
 
+// Division of 0 <= x < 2^31 by d: x m / 2^(31 + l) with m = 2^(31 + l) / d
+// rounded up and 2^l >= d, exact because x (m d - 2^(31 + l)) < 2^31 2^l.  The
+// hardware has no integer division.
+struct Div {
+  uint32_t m, s;
+  static Div by(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return Div{static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d), 31 + l};
+  }
+  __device__ __forceinline__ int operator()(int x) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * m >> s);
+  }
+};
+
 }  // namespace fmoe

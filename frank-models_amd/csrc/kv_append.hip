@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+constexpr int kMaxHeadDim = 128;
 constexpr int kVec = 8;           // elements of a lane's load
 constexpr int kBatch = 4;         // loads of a lane in flight
 constexpr int kAngleFloats = 8192;  // LDS for (cos, sin): rows of a chunk x head_dim
@@ -79,9 +80,15 @@ __device__ __forceinline__ void values8(u32x2_t c, float* x) {
   }
 }
 
-// The page of position 0 rounded down also for positions before the sequence.
-__device__ __forceinline__ int64_t first_page(int start, int block_size) {
-  return start >= 0 ? start / block_size : -((-static_cast<int64_t>(start) + block_size - 1) / block_size);
+struct Plan {
+  int pages;  // that a sequence's new tokens can touch
+  Div page_div, block_div;  // by pages, by block_size
+};
+
+// The page of a sequence's first new token, rounded down also for positions
+// before the sequence.
+__device__ __forceinline__ int first_page(const Plan& p, int start) {
+  return start >= 0 ? p.block_div(start) : -1 - p.block_div(-1 - start);
 }
 
 // The new tokens [lo, hi) of a sequence from `start` that lie in its page lp.
@@ -91,20 +98,25 @@ __device__ __forceinline__ void page_tokens(int64_t lp, int start, int seq_len, 
   hi = static_cast<int>(min(max(first + block_size, static_cast<int64_t>(0)), static_cast<int64_t>(seq_len)));
 }
 
+__device__ __forceinline__ double2 cmul(double2 a, double2 b) {
+  return double2{a.x * b.x - a.y * b.y, a.x * b.y + a.y * b.x};
+}
+
 // Block (page of the new tokens, group of heads, sequence).  An item is one
 // K, V or Q head of the page's new tokens; a wave takes an item, so a head's
 // maximum needs no barrier.  Bound by memory; for a decode step's few tokens
 // by one round trip after another (start, table entry, page scale).
 // T: activations.  C: codes (the pool holds e4m3), else the pool holds T.
 template <typename T, bool C>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a) {
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a, Plan plan) {
   extern __shared__ __attribute__((aligned(16))) float2 angles[];  // [rows of a chunk][D / 2]
+  __shared__ double2 turns[2][kMaxHeadDim / 2];
   const int b = blockIdx.z, x = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int D = 1 << a.log2_dim, bs = a.block_size;
   const int start = a.start[b];
   const int len = a.lens ? min(max(a.lens[b], 0), a.seq_len) : a.seq_len;  // tokens that are cached
-  const int64_t lp = first_page(start, bs) + x;
+  const int64_t lp = static_cast<int64_t>(first_page(plan, start)) + x;
   int s0, s1;
   page_tokens(lp, start, a.seq_len, bs, s0, s1);
   if (s0 >= s1) return;
@@ -120,16 +132,24 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a) {
   }
   bool later = false;
   if (page >= 0) {
-    const int64_t count = static_cast<int64_t>(a.batch - b) * a.pages;
-    for (int64_t i = x + 1 + tid; i < count; i += kThreads) {
-      const int b2 = b + static_cast<int>(i / a.pages);
+    // (b2, x2): sequence and page, kThreads pages on in each round
+    const int on = plan.page_div(kThreads), on_x = kThreads - on * plan.pages, skip = plan.page_div(tid);
+    int64_t x2 = static_cast<int64_t>(x) + 1 + tid - static_cast<int64_t>(skip) * plan.pages;
+    int b2 = b + skip;
+    while (true) {
+      if (x2 >= plan.pages) {
+        x2 -= plan.pages;
+        ++b2;
+      }
+      if (b2 >= a.batch) break;
       const int st2 = a.start[b2];
-      const int64_t lp2 = first_page(st2, bs) + i % a.pages;
-      if (lp2 < 0 || lp2 >= a.max_blocks) continue;
+      const int64_t lp2 = first_page(plan, st2) + x2;
       int lo, hi;
       page_tokens(lp2, st2, a.seq_len, bs, lo, hi);
-      if (lo >= hi || (a.lens && lo >= a.lens[b2])) continue;
-      later |= a.tables[static_cast<int64_t>(b2) * a.max_blocks + lp2] == page;
+      if (lp2 >= 0 && lp2 < a.max_blocks && lo < hi && (!a.lens || lo < a.lens[b2]))
+        later |= a.tables[static_cast<int64_t>(b2) * a.max_blocks + lp2] == page;
+      x2 += on_x;
+      b2 += on;
     }
   }
   const bool write = !__syncthreads_or(later) && page >= 0;
@@ -160,19 +180,25 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a) {
         const int c1 = min(c0 + chunk, n);
         if (a.rope && (!have_angles || chunk < n)) {  // block-uniform
           if (have_angles) __syncthreads();
-          // A thread keeps one pair and steps through rows: angles in 64 bits,
-          // the row's turned on by the step's with a complex product.
-          const int pairs = D / 2, i = tid & (pairs - 1), step = kThreads >> (a.log2_dim - 1);
-          const double freq = a.freq_scale * exp2(-static_cast<double>(2 * i) / D * a.log2_base);
-          const int r = tid >> (a.log2_dim - 1);
-          double sn, cs, dsn = 0., dcs = 1.;
-          sincos(static_cast<double>(static_cast<int64_t>(start) + s0 + c0 + r) * freq, &sn, &cs);
-          if (r + step < c1 - c0) sincos(static_cast<double>(step) * freq, &dsn, &dcs);
-          for (int row = r; row < c1 - c0; row += step) {
-            angles[row * pairs + i] = float2{static_cast<float>(cs), static_cast<float>(sn)};
-            const double t = cs * dcs - sn * dsn;
-            sn = sn * dcs + cs * dsn;
-            cs = t;
+          // A thread keeps one pair and steps through rows.  In 64 bits: one
+          // sine and cosine a pair for the chunk's first row and one for a
+          // row's step, and complex products for the rest.
+          const int log2_pairs = a.log2_dim - 1, i = tid & ((1 << log2_pairs) - 1), r = tid >> log2_pairs;
+          if (r < 2) {
+            const double freq = a.freq_scale * exp2(-static_cast<double>(2 * i) / D * a.log2_base);
+            double sn, cs;
+            sincos((r ? 1. : static_cast<double>(static_cast<int64_t>(start) + s0 + c0)) * freq, &sn, &cs);
+            turns[r][i] = double2{cs, sn};
+          }
+          __syncthreads();
+          double2 z = turns[1][i], w = turns[0][i];
+          for (int bit = 1; bit < kThreads >> log2_pairs; bit *= 2) {
+            if (r & bit) w = cmul(w, z);
+            z = cmul(z, z);
+          }
+          for (int row = r; row < c1 - c0; row += kThreads >> log2_pairs) {
+            angles[(row << log2_pairs) + i] = float2{static_cast<float>(w.x), static_cast<float>(w.y)};
+            w = cmul(w, z);
           }
           have_angles = true;
           __syncthreads();
@@ -261,25 +287,31 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a) {
 
 }  // namespace
 
-hipError_t launch_kv_append(const KvAppendArgs& args, int act, bool codes, hipStream_t s) {
-  KvAppendArgs a = args;
+hipError_t launch_kv_append(const KvAppendArgs& a, int act, bool codes, hipStream_t s) {
   if (a.batch == 0 || a.seq_len == 0) return hipSuccess;
   // pages that seq_len tokens from any start can touch
   const int64_t pages = (static_cast<int64_t>(a.seq_len) + a.block_size - 2) / a.block_size + 1;
-  a.pages = static_cast<int>(pages);
+  const Plan plan{static_cast<int>(pages), Div::by(static_cast<uint32_t>(pages)),
+                  Div::by(static_cast<uint32_t>(a.block_size))};
   const int items = 2 * a.n_head_kv + (a.q ? a.n_head : 0);
   const int groups = (items + kWaves - 1) / kWaves;
   const int rows = min(min(a.block_size, a.seq_len), kAngleFloats >> a.log2_dim);
   const size_t lds = a.rope ? (static_cast<size_t>(rows) << a.log2_dim) * sizeof(float) : 0;
-  const dim3 grid(static_cast<unsigned>(pages), groups, a.batch);
+    // About 1024 blocks, each with as many rounds of items: they share the
+  // page's angles and the search for later appends (us at 1024, 2048 and as
+  // many blocks as there are groups: TBD).
+  const int64_t pages_all = pages * a.batch, want = (1024 + pages_all - 1) / pages_all;
+  const int rounds = want < groups ? static_cast<int>((groups + want - 1) / want) : 1;
+  const int y = (groups + rounds - 1) / rounds;
+  const dim3 grid(static_cast<unsigned>(pages), y, a.batch);
   if (act == DT_F32 && codes)
-    hipLaunchKernelGGL((kv_append_kernel<float, true>), grid, dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((kv_append_kernel<float, true>), grid, dim3(kThreads), lds, s, a, plan);
   else if (act == DT_F32)
-    hipLaunchKernelGGL((kv_append_kernel<float, false>), grid, dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((kv_append_kernel<float, false>), grid, dim3(kThreads), lds, s, a, plan);
   else if (codes)
-    hipLaunchKernelGGL((kv_append_kernel<bf16_t, true>), grid, dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((kv_append_kernel<bf16_t, true>), grid, dim3(kThreads), lds, s, a, plan);
   else
-    hipLaunchKernelGGL((kv_append_kernel<bf16_t, false>), grid, dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((kv_append_kernel<bf16_t, false>), grid, dim3(kThreads), lds, s, a, plan);
   return hipGetLastError();
 }
 

@@ -426,7 +426,6 @@ struct KvAppendArgs {
   const int* lens;    // [batch] or null
   int64_t n_blocks;
   int block_size, max_blocks, batch, seq_len, n_head, n_head_kv, log2_dim;
-  int pages;  // set by the launcher: pages that a sequence's new tokens can touch
   int rope;
   double log2_base, freq_scale;
 };

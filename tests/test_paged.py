@@ -70,6 +70,38 @@ def test_attention_refuses(fm, kw, status):
     assert ll.lib().fmoe_attention_paged(*attn_args(ll, **kw)) == getattr(ll, status), ll.last_error()
 
 
+def step_args(ll, sublayer=False, **kw):
+    a = dict(x=FAKE, norm=FAKE, eps=1e-5) if sublayer else dict(x=FAKE)
+    a.update(positions=FAKE, k_cache=FAKE, v_cache=FAKE, k_scales=FAKE, v_scales=FAKE, n_blocks=8, block_size=4,
+             layer=0, tables=FAKE, context=FAKE, n_layers=1, max_blocks=4, max_context=16, blocks=FAKE, rows=FAKE,
+             wqkv=FAKE, wqkv_scales=None, wo=FAKE, wo_scales=None, w_dtype=ll.BF16, bq=None, bk=None, bv=None, bo=None,
+             use_bias=0, batch=2, n_head=4, n_head_kv=2, n_embd=64, n_embd_kv=32, base=1e4, scale=1.0, act=ll.BF16,
+             out=FAKE, k_new=FAKE, v_new=FAKE, workspace=FAKE, nbytes=1 << 40, stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("sublayer", [False, True])
+@pytest.mark.parametrize("kw,status", [
+    (dict(act=2), "ERR_DTYPE"), (dict(n_head=3), "ERR_SHAPE"), (dict(layer=1), "ERR_SHAPE"),
+    (dict(block_size=1 << 30), "ERR_SHAPE"), (dict(max_blocks=0), "ERR_SHAPE"),
+    (dict(max_context=(1 << 31) - 4096), "ERR_SHAPE"), (dict(max_context=-1), "ERR_SHAPE"),
+    (dict(k_scales=None), "ERR_INVALID_ARGUMENT"), (dict(v_scales=None), "ERR_INVALID_ARGUMENT"),
+    (dict(v_cache=None), "ERR_INVALID_ARGUMENT"), (dict(blocks=None), "ERR_INVALID_ARGUMENT"),
+    (dict(k_cache=FAKE + 8), "ERR_INVALID_ARGUMENT"), (dict(k_new=FAKE + 8), "ERR_INVALID_ARGUMENT"),
+    (dict(workspace=None), "ERR_INVALID_ARGUMENT"), (dict(nbytes=64), "ERR_WORKSPACE"),
+])
+def test_decode_step_refuses(fm, sublayer, kw, status):
+    ll = fm.lowlevel
+    fn = f"fmoe_attention_{'sublayer_' if sublayer else ''}decode_paged_f8"
+    assert getattr(ll.lib(), fn)(*step_args(ll, sublayer, **kw)) == getattr(ll, status), ll.last_error()
+    assert getattr(ll.lib(), fn)(*step_args(ll, sublayer, batch=0)) == ll.OK or sublayer
+    room = getattr(ll.lib(), fn + "_workspace_bytes")
+    assert room(2, 16, 4, 2, 64, 32, ll.BF16) > 0
+    for bad in ((-1, 16, 4, 2, 64, 32), (2, 1 << 31, 4, 2, 64, 32), (2, 16, 4, 3, 64, 32), (2, 16, 0, 2, 64, 32)):
+        assert room(*bad, ll.BF16) == 0
+
+
 def test_attention_workspace_is_checked(fm):
     """A decode step behind a long context is cut over blocks, whose partial results need room."""
     ll = fm.lowlevel
