@@ -219,6 +219,7 @@ constexpr int kSub = kChunk / 16;  // groups of 16 positions
 // grown by more than 2^kLazy: weights are then at most 2^kLazy, which fp32
 // sums and bf16 operands hold as well.
 constexpr float kLazy = 8.f;
+constexpr float kMaxSum = 256.f;  // a lane's sum of weights: each is below 2^kLazy
 
 template <int D>
 struct Stream {
@@ -629,18 +630,25 @@ __global__ __launch_bounds__(kThreads, 2) void paged_stream_kernel(PagedAttnArgs
 
 // ------------------------------------------------------------------ many rows
 // Block (row tile of 128, K/V head, context split; sequence): wave w has 32
-// rows, and the four share tiles of 64 positions, three in LDS: while one is
-// computed the next two are in flight (global_load_lds; one block barrier a
-// tile).  Bound by the matrix cores and, beside them, by the vector work of
-// the softmax; 64 positions of 32 rows are 1024 cycles of products at
-// head_dim 128 and about as many of vector instructions.
+// rows, and the four share tiles of 128 positions, two in LDS: while one is
+// computed the next is in flight (global_load_lds; one block barrier a tile).
 // Scores: v_mfma_scale_f32_32x32x64_f8f6f4 with A = the K codes as they lie
 // and B = q as two e4m3 terms under a power of two of the row: hi = e4m3(q/s),
 // lo = e4m3(q/s - hi), exact for bf16 values down to s/4 and within s/1024
 // below.  Two fp8 products cost what one bf16 product does and spare the
 // conversion of K.  A lane holds, for row l % 32, positions 8 i + 4 (l / 32)
 // + 0..3, which serve as the B operand of the second product in bf16
-// (32x32x16) with A = V transposed, converted as it is read.
+// (32x32x16) with A = V transposed, converted as it is read.  The denominator
+// adds the weights before they are rounded to bf16 (2^-8 of each, at most,
+// goes into the numerator); adding them as rounded, in v_dot2, waited for
+// every product in flight, which the other vector instructions pass by.
+// Bound by the matrix cores and the vector unit under the card's power: 64
+// positions of 32 rows are 1024 cycles of products and about 900 of vector
+// instructions at head_dim 128, which two waves overlap, but with every CU at
+// it the clock falls to 1.7 - 1.95 GHz (products alone: 1.75).  8192 tokens
+// of 8192, 32/8 heads x 128, causal: 533 us, 1.03 PFLOP/s where a library's
+// bf16 product of 8192^3 reaches 1.2; without the interleaving of products
+// and softmax 605.
 constexpr int kBigRows = 128;
 constexpr int kWaveRows = 32;
 constexpr int kBigTile = 128;
@@ -664,13 +672,6 @@ __device__ __forceinline__ u32x4_t scaled_bf16x8(uint32_t a, float s, uint32_t b
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, t, false)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, t, true))};
-}
-
-// s plus both halves of w.
-__device__ __forceinline__ float add_bf16x2(uint32_t w, float s) {
-  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-  const bf16x2_t one = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), one, s, false);
 }
 
 template <int D>
@@ -748,22 +749,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     k_at[i] = kp + ((lc ^ k_place<D>(i * R::kRowsPerLoad + lr)) << 4);
     v_at[i] = vp + ((lc ^ v_place32<D>(i * R::kRowsPerLoad + lr)) << 4);
   }
-  auto load_tile = [&](int stage) __attribute__((always_inline)) {
+  // A tile's loads: its rows (every lane's own position, then of each load),
+  // the entries of the tile after it and this one's scales, and load i.
+  struct Rows {
+    int page;
+    uint32_t r[R::kLoads];
+  };
+  auto load_rows = [&](int stage, Rows& rows) __attribute__((always_inline)) {
     const int entry = entries[lane];
     const bool in = next_j < end;
     const bool ok = (next_page < a.max_blocks) & (static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.n_blocks)) & in;
     const uint32_t valid = static_cast<uint32_t>(__ballot(ok)), zero = static_cast<uint32_t>(__ballot(in & !ok));
     // unusable rows load a usable one (row 0 is there)
-    const int from = valid ? __builtin_ctz(valid) : 0;
+    const int from = __builtin_ctz(valid | 1u << 31);
     const int some_page = valid ? __builtin_amdgcn_readlane(entry, from) : 0;
     const int some_off = valid ? __builtin_amdgcn_readlane(next_off, from) : 0;
-    const int page = ok ? entry : some_page;
-    const int use = page * a.block_size + (ok ? next_off : some_off);
-    unsigned char* base = lds + stage * R::kStageB;
+    rows.page = ok ? entry : some_page;
+    const int use = rows.page * a.block_size + (ok ? next_off : some_off);
     if (lane < 2) flags[stage * 2 * kWaves + kWaves * lane + wave] = lane ? zero : valid;
-    uint32_t r[R::kLoads];
 #pragma unroll
-    for (int i = 0; i < R::kLoads; ++i) r[i] = __shfl(use, i * R::kRowsPerLoad + lr, kWave);
+    for (int i = 0; i < R::kLoads; ++i) rows.r[i] = __shfl(use, i * R::kRowsPerLoad + lr, kWave);
+  };
+  auto load_scales = [&](int stage, const Rows& rows) __attribute__((always_inline)) {
     next_j += kBigTile;
     next_page += page_step;
     next_off += off_step;
@@ -771,15 +778,21 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     next_off -= wrap ? a.block_size : 0;
     next_page += wrap ? 1 : 0;
     load_entries();
-    load_lds4(scales_of + static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(a.n_head_kv),
-              base + 2 * R::kTileB + wave * kWave * 4);
+    load_lds4(scales_of + static_cast<uint64_t>(static_cast<uint32_t>(rows.page)) * static_cast<uint32_t>(a.n_head_kv),
+              lds + stage * R::kStageB + 2 * R::kTileB + wave * kWave * 4);
+  };
+  auto load_part = [&](int stage, const Rows& rows, int i) __attribute__((always_inline)) {
+    unsigned char* base = lds + stage * R::kStageB + (wave * R::kLoads + i) * 1024;
+    const uint64_t off = static_cast<uint64_t>(rows.r[i]) * row_b;
+    load_lds16_cached(k_at[i % kPlaces] + off, base);
+    load_lds16_cached(v_at[i % kPlaces] + off, base + R::kTileB);
+  };
+  auto load_tile = [&](int stage) __attribute__((always_inline)) {
+    Rows rows;
+    load_rows(stage, rows);
+    load_scales(stage, rows);
 #pragma unroll
-    for (int i = 0; i < R::kLoads; ++i) {
-      const uint64_t off = static_cast<uint64_t>(r[i]) * row_b;
-      const int at = (wave * R::kLoads + i) * 1024;
-      load_lds16_cached(k_at[i % kPlaces] + off, base + at);
-      load_lds16_cached(v_at[i % kPlaces] + off, base + R::kTileB + at);
-    }
+    for (int i = 0; i < R::kLoads; ++i) load_part(stage, rows, i);
   };
 
   // ---- q as two terms: lane (half, col) holds dimensions 64 s + 32 half + 0..31 of row col
@@ -831,6 +844,30 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
+  // K of 64 positions of a stage, by (32 positions, 64 dimensions), and the
+  // products of one, in both terms, times 2^(e8m0 - 127)
+  auto keys = [&](const unsigned char* base, int h64, i32x8_t (&k)[2][D / 64]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt) {
+        u32x4_t w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          w[e] = *reinterpret_cast<const u32x4_t*>(base + (64 * h64 + 32 * pt + col) * D +
+                                                   (((4 * s + 2 * half + e) ^ k_place<D>(col)) << 4));
+        k[pt][s] = __builtin_bit_cast(i32x8_t, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+  };
+  // V columns of 64 positions: v[s][d], 8 codes of positions 16 s + ...
+  auto columns = [&](const unsigned char* base, int h64, u32x2_t (&v)[4][D / 32]) __attribute__((always_inline)) {
+    const int k = (lane & 15) >> 1, r = 8 * (k >> 2) + 4 * half + (k & 3);  // and 16 s
+    const uint32_t row = lds_address(base + R::kTileB + (64 * h64 + r) * D + 8 * (lane & 1));
+    uint32_t from[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) from[d] = row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4);
+    read_columns4<16 * D>(from, v);
+  };
   int nan_from = INT32_MAX, nan_to = 0;  // positions among which V codes that are NaN were left out
   if (n > 0) {
     load_entries();
@@ -847,39 +884,132 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
-    if (t + 1 < n) load_tile(~t & 1);
-    const int at = j0 + t * kBigTile;
-    if (at >= wave_end) continue;  // none of this wave's rows
+    const bool more = t + 1 < n;
+    const int at = j0 + t * kBigTile, other = ~t & 1;
+    if (at >= wave_end) {  // none of this wave's rows
+      if (more) load_tile(other);
+      continue;
+    }
     const unsigned char* base = lds + (t & 1) * R::kStageB;
     const float* scales = reinterpret_cast<const float*>(base + 2 * R::kTileB);  // by wave: 32 of K, 32 of V
     const uint32_t* fl = flags + (t & 1) * 2 * kWaves;
-    uint32_t valid[kWaves], all = ~0u;
+    i32x8_t k0[2][D / 64];
+    keys(base, 0, k0);
+    float ks[kWaves];  // of position col of each 32
+    uint32_t su[kWaves], all = ~0u;  // scales of this lane's positions, K's and V's
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      valid[w] = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[w]));
-      all &= valid[w];
+      ks[w] = scales[w * kWave + col];
+      su[w] = __float_as_uint(scales[w * kWave + lane]);
+      all &= __builtin_amdgcn_readfirstlane(static_cast<int>(fl[w]));
     }
     const bool full = all == ~0u && at + kBigTile <= first_limit;
     // Scales that are powers of two, V's one for four neighbouring positions,
     // cost nothing: the products take K's, the conversion of V takes V's.
     // Others multiply scores and weights.
-    float ks[kWaves];  // of position col of each 32
+    const bool pow2 = plan.aligned && !__any(((su[0] | su[1] | su[2] | su[3]) & 0x7FFFFFu) |
+                                             (min(min(su[0], su[1]), min(su[2], su[3])) < 0x800000u) |
+                                             (max(max(su[0], su[1]), max(su[2], su[3])) >= 0x7F800000u));
+    // Tiles that every row attends, with scales that are powers of two, behind
+    // the first: 64 positions' products run beside the other 64's softmax, and
+    // the first 64's beside the next tile's loads.  Weights are taken against
+    // the maximum as it stands; where a lane's sum says that it has to be
+    // raised, the 64 positions are done again below.
+    int done = 0;
+    if (full && pow2 && !__any(m == -INFINITY)) {
+      const float mc = m * c2;
+      int e8m0[4];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) ks[w] = scales[w * kWave + col];
-    bool pow2 = plan.aligned;
-    if (pow2) {
-      uint32_t any = 0, least = ~0u, most = 0;
+      for (int w = 0; w < kWaves; ++w) e8m0[w] = static_cast<int>(__float_as_uint(ks[w]) >> 23);
+      f32x16_t sc[2][2];
+      u32x4_t p[2][4];
+      u32x2_t v[4][D / 32];
+      float w[2], vs[8], sums[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+      auto score = [&](int h64, const i32x8_t (&k)[2][D / 64], int i) __attribute__((always_inline)) {
+        const int pt = i & 1, s = i >> 2;
+        sc[h64][pt] = mfma32_f8(k[pt][s], e8m0[2 * h64 + pt], i & 2 ? ql[s] : qh[s], sc[h64][pt]);
+      };
+      // Weights 2 i and 2 i + 1 of 64 positions, after those before are added
+      // to the sums and rounded to bf16.
+      auto weigh = [&](int h64, int i) __attribute__((always_inline)) {
+        float next[2];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const uint32_t u = __float_as_uint(scales[w * kWave + lane]);
-        any |= u;
-        least = min(least, u);
-        most = max(most, u);
+        for (int e = 0; e < 2; ++e)
+          if (i < 16) next[e] = __builtin_amdgcn_exp2f(fmaf(sc[h64][i >> 3][2 * (i & 7) + e], c2, -mc));
+        if (i > 0) {
+          p[h64][(i - 1) >> 2][(i - 1) & 3] = pack_bf16x2(w[0], w[1]);
+          sums[h64][0] += w[0];
+          sums[h64][1] += w[1];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (i < 16) w[e] = next[e];
+      };
+      auto load_values = [&](int h64) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) vs[g] = scales[(2 * h64 + (g >> 2)) * kWave + 32 + 8 * (g & 3) + 4 * half];
+        columns(base, h64, v);
+      };
+      auto convert = [&](int i) __attribute__((always_inline)) {
+        const int s = i / (D / 32), d = i % (D / 32);
+        return scaled_bf16x8(v[s][d][0], vs[2 * s], v[s][d][1], vs[2 * s + 1]);
+      };
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[h][0][i] = sc[h][1][i] = 0.f;
+      Rows rows;
+      constexpr int kProducts = D / 16;
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        score(0, k0, i);
+        __builtin_amdgcn_sched_barrier(0);
+        // (behind the last tile, rows that nothing reads)
+        if (i == 0) load_rows(other, rows);
+        if (i == 1) load_scales(other, rows);
+        if (i >= 2 && i - 2 < R::kLoads) load_part(other, rows, i - 2);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      pow2 = !__any((any & 0x7FFFFFu) | (least < 0x800000u) | (most >= 0x7F800000u));
-    }
+      static_assert(kProducts - 2 >= R::kLoads, "every load has a product");
+      i32x8_t k1[2][D / 64];
+      keys(base, 1, k1);
+      asm volatile("" : "+v"(sc[0][0]), "+v"(sc[0][1]));
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int h64 = 0; h64 < 2; ++h64) {  // 64 positions at a time
+      for (int i = 0; i < 16; ++i) {
+        if (i % (256 / D) == 0) score(1, k1, i / (256 / D));
+        weigh(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      weigh(0, 16);
+      load_values(0);
+      // not moved behind the branch
+      asm volatile("" : "+v"(sc[1][0]), "+v"(sc[1][1]), "+v"(p[0][0]), "+v"(p[0][1]), "+v"(p[0][2]), "+v"(p[0][3]));
+      if (!__any(sums[0][0] + sums[0][1] > kMaxSum)) {
+        l += sums[0][0] + sums[0][1];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const u32x4_t c = convert(i % (D / 8));
+          weigh(1, i);
+          if (i < D / 8) acc[i % (D / 32)] = mfma32(c, p[0][i / (D / 32) % 4], acc[i % (D / 32)]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        weigh(1, 16);
+        done = 1;
+        if (!__any(sums[1][0] + sums[1][1] > kMaxSum)) {
+          l += sums[1][0] + sums[1][1];
+          load_values(1);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) acc[i % (D / 32)] = mfma32(convert(i), p[1][i / (D / 32)], acc[i % (D / 32)]);
+          done = 2;
+        }
+      }
+    } else if (more) {
+      load_tile(other);
+    }
+#pragma unroll 1
+    for (int h64 = done; h64 < 2; ++h64) {  // 64 positions at a time
       const int half_at = at + 64 * h64;
       if (half_at >= wave_end) break;
       float vs[8];  // of positions 8 g + 4 half + 0..3
@@ -896,30 +1026,25 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 #pragma unroll
         for (int pt = 0; pt < 2; ++pt) {
           const uint32_t below = static_cast<uint32_t>(low_bits(min(limit - half_at - 32 * pt, 32)));
-          on[pt] = (valid[2 * h64 + pt] & below) >> (4 * half);
+          on[pt] = (fl[2 * h64 + pt] & below) >> (4 * half);
           nil[pt] = (fl[kWaves + 2 * h64 + pt] & below) >> (4 * half);
         }
       }
 
       // ---- scores
       f32x16_t sc[2];
+      int e8m0[2];
 #pragma unroll
-      for (int pt = 0; pt < 2; ++pt) {
+      for (int pt = 0; pt < 2; ++pt)
+        e8m0[pt] = pow2 ? static_cast<int>(__float_as_uint(scales[(2 * h64 + pt) * kWave + col]) >> 23) : 127;
+      i32x8_t k[2][D / 64];
+      keys(base, h64, k);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[pt][i] = 0.f;
-        const int r = 64 * h64 + 32 * pt + col;
-        const int e8m0 = pow2 ? static_cast<int>(__float_as_uint(ks[2 * h64 + pt]) >> 23) : 127;
+      for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.f;
 #pragma unroll
-        for (int s = 0; s < D / 64; ++s) {
-          u32x4_t w[2];
+      for (int s = 0; s < D / 64; ++s)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            w[e] = *reinterpret_cast<const u32x4_t*>(base + r * D + (((4 * s + 2 * half + e) ^ k_place<D>(r)) << 4));
-          const i32x8_t k = __builtin_bit_cast(i32x8_t, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
-          sc[pt] = mfma32_f8(k, e8m0, qh[s], sc[pt]);
-          sc[pt] = mfma32_f8(k, e8m0, ql[s], sc[pt]);
-        }
-      }
+        for (int i = 0; i < 4; ++i) sc[i & 1] = mfma32_f8(k[i & 1][s], e8m0[i & 1], i & 2 ? ql[s] : qh[s], sc[i & 1]);
       if (!pow2) {
 #pragma unroll
         for (int pt = 0; pt < 2; ++pt)
@@ -957,51 +1082,40 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
       }
       const float mc = finite_base(m) * c2;
       u32x4_t p[4];
-      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+      float sums[2] = {0.f, 0.f};
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt) {
         float w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(sc[pt][i], c2, -mc));
+        for (int i = 0; i < 16; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(fmaf(sc[pt][i], c2, -mc));
+          sums[i & 1] += w[i];
+        }
         if (!pow2) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            sums[i & 3] += w[i];
             w[i] *= scales[(2 * h64 + pt) * kWave + 32 + 8 * (i >> 2) + 4 * half + (i & 3)];
             if (!(on[pt] & 1u << (8 * (i >> 2) + (i & 3)))) w[i] = 0.f;  // 0 times a scale that is not finite
           }
         }
         split8<1>(w, &p[2 * pt]);
         split8<1>(w + 8, &p[2 * pt + 1]);
-        if (pow2) {  // the sum of the weights as they are multiplied, rounded to bf16
+        if (pow2 && !full) {  // a row of zeros has its weight and no value
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[e] = add_bf16x2(p[2 * pt + g][e], sums[e]);
-          if (!full) {  // a row of zeros has its weight and no value
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t bits = on[pt] >> (8 * (2 * g + (e >> 1)) + 2 * (e & 1));
-                p[2 * pt + g][e] &= (bits & 1 ? 0xFFFFu : 0u) | (bits & 2 ? 0xFFFF0000u : 0u);
-              }
-          }
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t bits = on[pt] >> (8 * (2 * g + (e >> 1)) + 2 * (e & 1));
+              p[2 * pt + g][e] &= (bits & 1 ? 0xFFFFu : 0u) | (bits & 2 ? 0xFFFF0000u : 0u);
+            }
         }
       }
-      l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      l += sums[0] + sums[1];
       __builtin_amdgcn_sched_barrier(0);
 
       // ---- values
       u32x2_t v[4][D / 32];
-      {
-        const int k = (lane & 15) >> 1, r = 64 * h64 + 8 * (k >> 2) + 4 * half + (k & 3);  // and 16 s
-        const uint32_t row = lds_address(base + R::kTileB + r * D + 8 * (lane & 1));
-        uint32_t from[D / 32];
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) from[d] = row + (((2 * d + (lane >> 4 & 1)) ^ v_place32<D>(r)) << 4);
-        read_columns4<16 * D>(from, v);
-      }
+      columns(base, h64, v);
       if (!full) {
         uint32_t any = 0;
 #pragma unroll
