@@ -435,6 +435,39 @@ def test_many_rows_extreme_sizes_and_queries(fm, monkeypatch):
     test_queries_that_are_not_finite_stay_in_their_rows(fm)
 
 
+@pytest.mark.parametrize("D,S,B", [(128, 70, 1), (64, 70, 1), (128, 256, 10)])
+def test_many_rows_maximum_is_raised_late(fm, D, S, B):
+    """Scales that are powers of two, and scores that outgrow all before them
+    in the first and the second half of a tile, in later tiles, by little and
+    by far; and codes that are NaN, for the rows that attend them."""
+    rng = np.random.default_rng(D + S)
+    H, Hkv, bs, ctx = 8, 4, 16, 900
+    per = -(-ctx // bs)
+    table = rng.permutation(B * per).reshape(B, per)
+    (kc, ks), (vc, vs) = (random_pool(rng, B * per, bs, Hkv, D) for _ in range(2))
+    ks, vs = (np.exp2(np.round(np.log2(s))).astype(np.float32) for s in (ks, vs))
+    for b in range(B):
+        for position, grow in ((130, 2), (200, 8), (390, 3), (450, 64), (520, 8)):
+            kc[table[b, position // bs], position % bs] = 0x70  # 128 in every dimension
+            ks[table[b, position // bs]] = 2.0 ** -12 * grow
+    q = rounded(rng.uniform(0.1, 1, (B, S, H, D)), "bf16")
+    limit = max(ctx, (13 << 20) // (B * S * H))
+    lens, dt = np.full((1, B), ctx, np.int32), dev(table[None].astype(np.int32))
+    call = lambda: fm.attention_paged(dev(q, "bf16"), gpu_pool(fm, kc, ks), gpu_pool(fm, vc, vs), 0, dt, dev(lens),  # noqa: E731
+                                      limit).double().cpu().numpy()
+    got = call()
+    ref, parts = op.attention(q, op.values(kc, ks), op.values(vc, vs), table, lens[0], limit, np.full(B, S))
+    assert np.all(np.abs(got - ref) <= op.attention_tolerance(ref, parts, D, "bf16"))
+    for j, h, d in ((140, 1, 5), (200, 0, D - 1), (700, 3, 0)):
+        vc[table[0, j // bs], j % bs, h, d] = 0xFF
+    hit = np.zeros((S, H, D), bool)  # token s attends positions to ctx - S + s
+    for j, h, d in ((140, 1, 5), (200, 0, D - 1), (700, 3, 0)):
+        hit[max(0, j - ctx + S) :, h * (H // Hkv) : (h + 1) * (H // Hkv), d] = True
+    new = call()
+    assert np.isnan(new[0][hit]).all() and np.array_equal(new[0][~hit], got[0][~hit])
+    assert np.array_equal(new[1:], got[1:])
+
+
 # ---------------------------------------------------------------- a run of both
 @pytest.mark.parametrize("act", ["bf16", "f32"])
 def test_prompt_then_decode(fm, act):
