@@ -1371,7 +1371,7 @@ hipError_t launch_attn(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     asked.fetch_or(bit, std::memory_order_relaxed);
   }
   const int64_t x = static_cast<int64_t>(p.tile_groups) * a.batch * p.n_split;
-  if (x > INT32_MAX) return hipErrorInvalidValue;  // the entry points bound it
+  if (x > UINT32_MAX / kThreads) return hipErrorInvalidValue;  // a grid counts its threads in 32 bits
   hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(x)), dim3(kThreads), kLds, s, a, p);
   return hipGetLastError();
 }

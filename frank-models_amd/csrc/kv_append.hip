@@ -21,27 +21,33 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxHeadDim = 128;
 constexpr int kVec = 8;           // elements of a lane's load
-constexpr int kBatch = 4;         // loads of a lane in flight
 constexpr int kAngleFloats = 8192;  // LDS for (cos, sin): rows of a chunk x head_dim
 
+// Eight elements as they lie.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
+struct Vec;
+template <>
+struct Vec<bf16_t> {
+  u32x4_t w;
+  __device__ __forceinline__ void get(float* x) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = bf16_lo(w[i]);
+      x[2 * i + 1] = bf16_hi(w[i]);
+    }
+  }
+};
+template <>
+struct Vec<float> {
+  f32x4_t a, b;
+  __device__ __forceinline__ void get(float* x) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[i] = a[i];
       x[4 + i] = b[i];
     }
-  } else {
-    const u32x4_t a = *reinterpret_cast<const u32x4_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = bf16_lo(a[i]);
-      x[2 * i + 1] = bf16_hi(a[i]);
-    }
   }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* x) {
@@ -104,10 +110,12 @@ __device__ __forceinline__ double2 cmul(double2 a, double2 b) {
 
 // Block (page of the new tokens, group of heads, sequence).  An item is one
 // K, V or Q head of the page's new tokens; a wave takes an item, so a head's
-// maximum needs no barrier.  Bound by memory; for a decode step's few tokens
-// by one round trip after another (start, table entry, page scale).
+// maximum needs no barrier.  Bound by memory: 4 x 2048 tokens of 32/8 heads x
+// 128 in bf16 to codes in pages of 32, 184 MB, take 37.6 us, 4.9 TB/s where a
+// copy reaches 5.2; for a decode step's few tokens by one round trip after
+// another: start, table entry, page scale (61 tokens 7.1 us).
 // T: activations.  C: codes (the pool holds e4m3), else the pool holds T.
-template <typename T, bool C>
+template <typename T, bool C, int kBatch>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a, Plan plan) {
   extern __shared__ __attribute__((aligned(16))) float2 angles[];  // [rows of a chunk][D / 2]
   __shared__ double2 turns[2][kMaxHeadDim / 2];
@@ -171,13 +179,58 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a, Pla
     const T* src = static_cast<const T*>(kind == 0 ? a.k : kind == 1 ? a.v : a.q) +
                    (static_cast<int64_t>(b) * a.seq_len + s0) * stride + (static_cast<int64_t>(head) << a.log2_dim);
     float amax = 0.f, inv = 0.f;
-    float v[kBatch][kVec];
+    Vec<T> raw[kBatch];
 
     // Two passes over the rows of a K or V item with codes (maximum, then
     // codes), one otherwise.
     for (int pass = C ? 0 : 1; pass < 2; ++pass) {
       for (int c0 = 0; c0 < n; c0 += chunk) {
         const int c1 = min(c0 + chunk, n);
+        const int vecs = max(min(c1, rows) - c0, 0) << log2_vecs;
+        const bool once = C && rows <= chunk && vecs <= kBatch * kWave;  // raw holds the rows through both passes
+        // A lane's load u of a batch from e0 on; lanes behind the last load take it too.
+        auto load = [&](int e0) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int e = min(e0 + u * kWave + lane, vecs - 1);
+            raw[u] = *reinterpret_cast<const Vec<T>*>(src + (c0 + (e >> log2_vecs)) * stride +
+                                                      ((e & ((1 << log2_vecs) - 1)) << 3));
+          }
+        };
+        auto work = [&](int e0) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int e = min(e0 + u * kWave + lane, vecs - 1);
+            const int row = c0 + (e >> log2_vecs), col = (e & ((1 << log2_vecs) - 1)) << 3;
+            float v[kVec];
+            raw[u].get(v);
+            if (turn) {
+              const float2* cs = angles + 4 * e;  // row e >> log2_vecs, pairs from 4 * (e's load of the row): 4 e in all
+#pragma unroll
+              for (int p = 0; p < 4; ++p) rope_apply(v[2 * p], v[2 * p + 1], cs[p], v[2 * p], v[2 * p + 1]);
+            }
+            if (pass == 0) {
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) {
+                const float m = fabsf(v[k]);
+                amax = fmaxf(amax, m < INFINITY ? m : 0.f);
+              }
+            } else if (kind == 2) {
+              store8(static_cast<T*>(a.q_out) + (static_cast<int64_t>(b) * a.seq_len + s0 + row) * a.q_out_stride +
+                         (static_cast<int64_t>(head) << a.log2_dim) + col,
+                     v);
+            } else {
+              const int64_t at = (page * bs + r0 + row) * row_elems + (static_cast<int64_t>(head) << a.log2_dim) + col;
+              void* pool = kind == 0 ? a.k_cache : a.v_cache;
+              if constexpr (C)
+                *reinterpret_cast<u32x2_t*>(static_cast<f8_t*>(pool) + at) = codes8(v, inv);
+              else
+                store8(static_cast<T*>(pool) + at, v);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // four waves a SIMD: one load's values at a time (37.6 us against 42.4)
+          }
+        };
+        if (vecs > 0 && !(once ? pass == 1 : pass == 0 && kind == 2)) load(0);  // before the angles, which take as long
         if (a.rope && (!have_angles || chunk < n)) {  // block-uniform
           if (have_angles) __syncthreads();
           // A thread keeps one pair and steps through rows.  In 64 bits: one
@@ -203,56 +256,10 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a, Pla
           have_angles = true;
           __syncthreads();
         }
-        const int vecs = max(min(c1, rows) - c0, 0) << log2_vecs;
         if (pass == 0 && kind == 2) continue;
-        const bool kept = C && kind != 2 && pass == 1 && rows <= chunk && vecs <= kBatch * kWave;  // v holds the rows
         for (int e0 = 0; e0 < vecs; e0 += kBatch * kWave) {
-          if (!kept) {
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-              const int e = e0 + u * kWave + lane;
-              if (e < vecs)
-                load8(src + (c0 + (e >> log2_vecs)) * stride + ((e & ((1 << log2_vecs) - 1)) << 3), v[u]);
-            }
-            if (turn) {
-#pragma unroll
-              for (int u = 0; u < kBatch; ++u) {
-                const int e = e0 + u * kWave + lane;
-                if (e < vecs) {
-                  // row e >> log2_vecs, pairs from 4 * (e's load of the row): 4 e in all
-                  const float2* cs = angles + 4 * e;
-#pragma unroll
-                  for (int p = 0; p < 4; ++p) rope_apply(v[u][2 * p], v[u][2 * p + 1], cs[p], v[u][2 * p], v[u][2 * p + 1]);
-                }
-              }
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const int e = e0 + u * kWave + lane;
-            if (e >= vecs) continue;
-            if (pass == 0) {
-#pragma unroll
-              for (int k = 0; k < kVec; ++k) {
-                const float m = fabsf(v[u][k]);
-                amax = fmaxf(amax, m < INFINITY ? m : 0.f);
-              }
-              continue;
-            }
-            const int row = c0 + (e >> log2_vecs), col = (e & ((1 << log2_vecs) - 1)) << 3;
-            if (kind == 2) {
-              store8(static_cast<T*>(a.q_out) + (static_cast<int64_t>(b) * a.seq_len + s0 + row) * a.q_out_stride +
-                         (static_cast<int64_t>(head) << a.log2_dim) + col,
-                     v[u]);
-              continue;
-            }
-            const int64_t at = (page * bs + r0 + row) * row_elems + (static_cast<int64_t>(head) << a.log2_dim) + col;
-            void* pool = kind == 0 ? a.k_cache : a.v_cache;
-            if constexpr (C)
-              *reinterpret_cast<u32x2_t*>(static_cast<f8_t*>(pool) + at) = codes8(v[u], inv);
-            else
-              store8(static_cast<T*>(pool) + at, v[u]);
-          }
+          if (e0 > 0) load(e0);
+          work(e0);
         }
       }
       if constexpr (C) {
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a, Pla
               const float f = old / scale;
               f8_t* pool = static_cast<f8_t*>(kind == 0 ? a.k_cache : a.v_cache) + page * bs * row_elems +
                            (static_cast<int64_t>(head) << a.log2_dim);
-              for (int e = lane; e < r0 << log2_vecs; e += kWave) {
+              for (int64_t e = lane; e < static_cast<int64_t>(r0) << log2_vecs; e += kWave) {
                 u32x2_t* p = reinterpret_cast<u32x2_t*>(pool + (e >> log2_vecs) * row_elems +
                                                         ((e & ((1 << log2_vecs) - 1)) << 3));
                 float y[kVec];
@@ -293,25 +300,38 @@ hipError_t launch_kv_append(const KvAppendArgs& a, int act, bool codes, hipStrea
   const int64_t pages = (static_cast<int64_t>(a.seq_len) + a.block_size - 2) / a.block_size + 1;
   const Plan plan{static_cast<int>(pages), Div::by(static_cast<uint32_t>(pages)),
                   Div::by(static_cast<uint32_t>(a.block_size))};
+  if (pages > UINT32_MAX / kThreads) return hipErrorInvalidValue;  // a grid counts its threads in 32 bits
   const int items = 2 * a.n_head_kv + (a.q ? a.n_head : 0);
   const int groups = (items + kWaves - 1) / kWaves;
   const int rows = min(min(a.block_size, a.seq_len), kAngleFloats >> a.log2_dim);
   const size_t lds = a.rope ? (static_cast<size_t>(rows) << a.log2_dim) * sizeof(float) : 0;
     // About 1024 blocks, each with as many rounds of items: they share the
-  // page's angles and the search for later appends (us at 1024, 2048 and as
-  // many blocks as there are groups: TBD).
+  // page's angles and the search for later appends (32/8 heads x 128, for 1024
+  // blocks, 2048 and one for each group, in us: 4 x 2048 tokens to pages of 32
+  // 37.6, 39.6, 41.5; 4 x 509 to bf16 pages of 16 12.3, 13.5, 13.5).
   const int64_t pages_all = pages * a.batch, want = (1024 + pages_all - 1) / pages_all;
   const int rounds = want < groups ? static_cast<int>((groups + want - 1) / want) : 1;
   const int y = (groups + rounds - 1) / rounds;
   const dim3 grid(static_cast<unsigned>(pages), y, a.batch);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, s, a, plan); };
+  // Loads of a lane in flight: as many as the rows of a page give it, so that
+  // K and V are read once and a page does not take one load's latency after
+  // another; no more, since each is computed (61 single tokens 7.1 us with 1,
+  // 10.1 with 4, 12.5 with 8; pages of 16 rows 12.0 with 4, 14.7 with 8; pages
+  // of 32 37.6 with 8, 45.5 with 4).
+  const int loads = ((rows << (a.log2_dim - 3)) + kWave - 1) / kWave;
   if (act == DT_F32 && codes)
-    hipLaunchKernelGGL((kv_append_kernel<float, true>), grid, dim3(kThreads), lds, s, a, plan);
+    launch(loads <= 1 ? kv_append_kernel<float, true, 1> : kv_append_kernel<float, true, 4>);
   else if (act == DT_F32)
-    hipLaunchKernelGGL((kv_append_kernel<float, false>), grid, dim3(kThreads), lds, s, a, plan);
+    launch(loads <= 1 ? kv_append_kernel<float, false, 1> : kv_append_kernel<float, false, 4>);
   else if (codes)
-    hipLaunchKernelGGL((kv_append_kernel<bf16_t, true>), grid, dim3(kThreads), lds, s, a, plan);
+    launch(loads <= 1   ? kv_append_kernel<bf16_t, true, 1>
+           : loads <= 4 ? kv_append_kernel<bf16_t, true, 4>
+                        : kv_append_kernel<bf16_t, true, 8>);
   else
-    hipLaunchKernelGGL((kv_append_kernel<bf16_t, false>), grid, dim3(kThreads), lds, s, a, plan);
+    launch(loads <= 1   ? kv_append_kernel<bf16_t, false, 1>
+           : loads <= 4 ? kv_append_kernel<bf16_t, false, 4>
+                        : kv_append_kernel<bf16_t, false, 8>);
   return hipGetLastError();
 }
 
