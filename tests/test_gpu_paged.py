@@ -468,6 +468,40 @@ def test_many_rows_maximum_is_raised_late(fm, D, S, B):
     assert np.array_equal(new[1:], got[1:])
 
 
+def test_pools_of_more_than_32_bits(fm):
+    """Pages past 4 GiB of a pool: appended to, and attended by one token, by
+    many, and by a decode step."""
+    rng = np.random.default_rng(41)
+    H, Hkv, D, bs, used = 16, 8, 128, 16, 30
+    n_blocks = (1 << 18) + used  # of 16 KiB
+    first = n_blocks - used
+    pools, small = [], []
+    for _ in range(2):
+        c, s = random_pool(rng, used, bs, Hkv, D)
+        p = fm.QuantizedKVPool(torch.empty((n_blocks, bs, Hkv, D), dtype=torch.uint8, device="cuda"),
+                               torch.empty((n_blocks, Hkv), device="cuda"))
+        p.data[first:], p.scales[first:] = dev(c), dev(s)
+        pools.append(p)
+        small.append(fm.QuantizedKVPool(dev(c), dev(s)))
+    table = rng.permutation(used).reshape(1, 1, used)
+    far, near = dev((table + first).astype(np.int32)), dev(table.astype(np.int32))
+    x = dev(rng.standard_normal((1, 60, H + 2 * Hkv, D)), "bf16")
+    start, context = dev(np.array([405], np.int32)), dev(np.array([[465]], np.int32))
+    blk, _ = block(fm, rng, "bf16", H, Hkv, D)
+    step = dev(rng.standard_normal((1, H * D)), "bf16")
+
+    def run(p, bt):
+        q, k, v = x.split([H, Hkv, Hkv], dim=2)
+        q = fm.kvcache_append(*p, 0, k, v, bt, start, q=q)
+        out = [q, fm.attention_paged(q[:, -1:], *p, 0, bt, context, 480), fm.attention_paged(q, *p, 0, bt, context, 480),
+               fm.attention_paged(q, *p, 0, bt, context, 1 << 15)]  # the kernel for many rows
+        return out + list(blk.paged(step, context[0].long(), *p, 0, bt, context, 465, bt[0, :, 29], context[0] % bs))
+
+    assert all(torch.equal(a, b) for a, b in zip(run(pools, far), run(small, near)))
+    for p, s in zip(pools, small):
+        assert torch.equal(p.data[first:], s.data) and torch.equal(p.scales[first:], s.scales)
+
+
 # ---------------------------------------------------------------- a run of both
 @pytest.mark.parametrize("act", ["bf16", "f32"])
 def test_prompt_then_decode(fm, act):
