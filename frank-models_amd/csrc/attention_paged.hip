@@ -8,6 +8,7 @@
 // Query rows of a K/V head are its (token, query head) pairs, token-major:
 // row r is token r / G, query head kvh * G + r % G, for G query heads per
 // K/V head, so that one read of K and V serves the group and the tokens.
+#include <algorithm>
 #include <atomic>
 
 #include "common.h"
@@ -1301,9 +1302,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, P
 // The kernel for many rows where (row, position) pairs are at least 12 M and a
 // K/V head has 32 rows: below, most of its 128-row blocks' time is latency,
 // and the other's 16-row tiles fill the GPU (4 query heads x 128, 8 K/V heads;
-// few rows against many rows: 512 tokens of 512 16.6 against 27.4 us, 128 of 2048
-// 26.5 and 27.7, 64 of 8192 44.1 and 35.7, 8 x 256 of 256 35.0 and 22.2, 8 x 8
-// of 8192 51.6 and 46.4).
+// few rows against many rows: 512 tokens of 512 16.1 against 28.0 us, 128 of 2048
+// 26.6 and 25.9, 64 of 8192 41.5 and 32.8, 8 x 256 of 256 34.5 and 22.9, 8 x 8
+// of 8192 44.0 and 42.2).
 constexpr double kBigPairs = 12 << 20;
 constexpr int kBigFrom = 32;
 
@@ -1321,9 +1322,12 @@ Plan plan_of(int batch, int seq_len, int max_ctx, int n_head, int n_head_kv, int
     p.waves_per_tile = 1;
     blocks = pairs * ((rows + kBigRows - 1) / kBigRows);
     n = 512 / blocks;
-    // Two splits of causal prompts are not worth joining (1024 tokens of 1024:
-    // 48 against 38 us with one).
-    if (n == 2 && max_ctx < 4ll * seq_len) n = 1;
+    // Splits of 512 positions at least (256 tokens of 2048 30.0 us with them,
+    // 32.0 with shorter ones, 35.8 with 1024; 8 x 128 of 512 23.5 and 36.0), and
+    // two only where there is much to halve (8 x 128 of 2048: 53.4 us with one,
+    // 61.2 with two; of 8192 165 and 156).
+    n = std::min<int64_t>(n, max_ctx / 512);
+    if (n == 2 && max_ctx < 4096) n = 1;
     quantum = 2 * kBigTile;
   } else {
     // About 1024 waves, one per SIMD, which keep the memory as busy as twice
