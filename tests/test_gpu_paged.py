@@ -468,6 +468,31 @@ def test_many_rows_maximum_is_raised_late(fm, D, S, B):
     assert np.array_equal(new[1:], got[1:])
 
 
+@pytest.mark.parametrize("low", [3.0, 8.0, 14.0, 40.0, 400.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_rows_scores_far_below_zero(fm, D, low):
+    """Scales that are powers of two, and scores of about -low: in all
+    positions, in the first tile alone, and in all but the last tokens'."""
+    rng = np.random.default_rng(int(low))
+    B, S, H, Hkv, bs, ctx = 1, 64, 4, 1, 16, 640
+    per = ctx // bs
+    table = rng.permutation(per)[None]
+    (_, ks), (vc, vs) = (random_pool(rng, per, bs, Hkv, D) for _ in range(2))
+    vs = np.exp2(np.round(np.log2(vs))).astype(np.float32)
+    q = rounded(rng.uniform(0.5, 1.5, (B, S, H, D)), "bf16")
+    limit, dt = (13 << 20) // (B * S * H), dev(table[None].astype(np.int32))
+    for span in ((0, ctx), (0, 128), (0, 600), (64, 200)):
+        want = rng.standard_normal((ctx, Hkv, D)) * 0.5
+        want[span[0] : span[1]] -= low * D ** -0.5
+        ks[:] = 2.0 ** np.ceil(np.log2((low * D ** -0.5 + 3) / 448))
+        kc = np.zeros((per, bs, Hkv, D), np.uint8)
+        kc[table[0]] = nm.e4m3fn_encode(want.reshape(per, bs, Hkv, D) / ks[0, 0])
+        got = fm.attention_paged(dev(q, "bf16"), gpu_pool(fm, kc, ks), gpu_pool(fm, vc, vs), 0, dt,
+                                 dev(np.array([[ctx]], np.int32)), limit).double().cpu().numpy()
+        ref, parts = op.attention(q, op.values(kc, ks), op.values(vc, vs), table, [ctx], limit, [S])
+        assert np.all(np.abs(got - ref) <= op.attention_tolerance(ref, parts, D, "bf16")), span
+
+
 def test_pools_of_more_than_32_bits(fm):
     """Pages past 4 GiB of a pool: appended to, and attended by one token, by
     many, and by a decode step."""
