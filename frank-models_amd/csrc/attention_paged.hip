@@ -805,7 +805,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     for (int i = 0; i < R::kLoads; ++i) load_part(stage, rows, i);
   };
 
-  // ---- q as two terms: lane (half, col) holds dimensions 64 s + 32 half + 0..31 of row col
+  // ---- q as two terms: lane (half, col) holds dimensions 64 s + 32 half + 0..31
+  // of row col.  Asked for beside the first tile's table entries, and
+  // converted (some 500 instructions) while that tile is loaded.
+  if (n > 0) load_entries();
   i32x8_t qh[D / 64], ql[D / 64];
   float c2, q_scale;
   {
@@ -815,11 +818,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
 #pragma unroll
     for (int s = 0; s < D / 64; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[s][i] = u32x4_t{0u, 0u, 0u, 0u};
-        if (token < span.len)
+      for (int i = 0; i < 4; ++i) w[s][i] = u32x4_t{0u, 0u, 0u, 0u};
+    if (token < span.len) {
+#pragma unroll
+      for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
           w[s][i] = *reinterpret_cast<const u32x4_t*>(static_cast<const bf16_t*>(a.q) + at + 64 * s + 32 * half + 8 * i);
-      }
+    }
+    __builtin_amdgcn_s_waitcnt(wait_vm(0, true));
+    asm volatile("" ::: "memory");
+    if (n > 0) load_tile(0);
 #pragma unroll
     for (int s = 0; s < D / 64; ++s)
 #pragma unroll
@@ -879,12 +888,6 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(PagedAttnArgs a
     read_columns4<16 * D>(from, v);
   };
   int nan_from = INT32_MAX, nan_to = 0;  // positions among which V codes that are NaN were left out
-  if (n > 0) {
-    load_entries();
-    __builtin_amdgcn_s_waitcnt(wait_vm(0, true));
-    asm volatile("" ::: "memory");
-    load_tile(0);
-  }
   for (int t = 0; t < n; ++t) {
     // This wave's part of tile t is there, and the next tile's table entries,
     // and so is everyone's part after the barrier, which no wave passes
